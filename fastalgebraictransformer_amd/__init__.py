@@ -38,6 +38,12 @@ from .backward import (
     rational_attention_masked,
     rational_attention_packed,
 )
+from .kv_cache import (
+    kv_cache_evict,
+    rational_attention_decode_accumulate,
+    rational_attention_key_weights,
+    rational_attention_tree,
+)
 from .algebraic_model import (
     AlgebraicAttention,
     AlgebraicBlock,
@@ -78,7 +84,9 @@ __all__ = [
 # norm that reads it; rational_attention_masked / MaskedRationalAttentionFunction,
 # attention with a key padding mask and a real non-causal mode;
 # rational_attention_decode, one query against a KV cache (the model's
-# generate() uses it).
+# generate() uses it); over the same caches rational_attention_tree (drafted
+# tokens), rational_attention_decode_accumulate, rational_attention_key_weights
+# and kv_cache_evict (a cache bounded by attention weight).
 
 
 def install_as(name="kernels"):
@@ -86,6 +94,6 @@ def install_as(name="kernels"):
     reference's package name ``kernels``) in ``sys.modules``."""
     pkg = _sys.modules[__name__]
     _sys.modules[name] = pkg
-    for sub in ("fused_ops", "forward", "backward", "algebraic_model"):
+    for sub in ("fused_ops", "forward", "backward", "kv_cache", "algebraic_model"):
         _sys.modules[f"{name}.{sub}"] = _sys.modules[f"{__name__}.{sub}"]
     return pkg

@@ -57,6 +57,18 @@ _SIGNATURES = {
                          _F, _INT, _P], _INT),
     "kat_attn_decode_noalloc": ([_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64P, _F, _F,
                                  _INT, _P], _INT),
+    "kat_attn_tree_workspace_size": ([_I64, _I64, _I64, _I64, _I64, _INT], _SZ),
+    "kat_attn_tree": ([_P, _P, _P, _P, _P, _P, _P, _I64, _P, _P, _I64P, _P, _SZ, _I64, _I64, _I64,
+                       _I64, _I64, _I64P, _F, _F, _INT, _P], _INT),
+    "kat_attn_decode_accum_workspace_size": ([_I64, _I64, _I64, _I64, _INT], _SZ),
+    "kat_attn_decode_accum": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64P, _P, _SZ, _I64, _I64,
+                               _I64, _I64, _I64P, _F, _F, _INT, _P], _INT),
+    "kat_attn_key_weights_workspace_size": ([_I64, _I64, _I64, _I64, _I64, _INT], _SZ),
+    "kat_attn_key_weights": ([_P, _P, _P, _P, _P, _P, _I64, _P, _SZ, _I64, _I64, _I64, _I64, _I64,
+                              _I64P, _F, _F, _INT, _P], _INT),
+    "kat_kv_evict_workspace_size": ([_I64, _I64, _I64], _SZ),
+    "kat_kv_evict": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _I64, _I64, _I64, _I64,
+                      _I64, _I64, _INT, _I64P, _INT, _P], _INT),
     "kat_probe_mfma_bf16": ([_P, _INT, _INT, ctypes.POINTER(ctypes.c_double), _P], _INT),
     "kat_probe_mfma_bf16_random": ([_P, _INT, _INT, ctypes.POINTER(ctypes.c_double), _P], _INT),
 }

@@ -1,0 +1,324 @@
+// The attention weight that each key of a prompt receives, summed over the
+// queries, on gfx950:
+//   w_j = sum_{i >= j, i >= T - last} f_ij / (L_i + eps),   f_ij = sigma(s_ij)^4,
+//   s_ij = scale <q_i, k_j> - slope_h (i - j)
+// with L the row sums that the forward (kat_attn_fwd) stored. With a token mask,
+// a dropped token neither gives nor receives weight. This is what an eviction
+// policy needs of a prompt before its keys go into a smaller cache.
+//
+// Design (MI355X). One matrix product and ~9 VALU operations per (query, key)
+// pair and no output but T floats per head: instruction issue (MFMA + VALU)
+// bounds it, not memory. Like the backward's dK/dV pass a block keeps its keys'
+// fragments in registers and streams the queries through LDS (64-row tiles,
+// double-buffered LDS-DMA, the swizzled tiles of attn_mfma_dev.h):
+//   S[q][key] = Q K^T   A = Q rows (ds_read_b128), B = K (registers)
+// and a lane holds queries 4 g + j of its key li, so the column sums stay in
+// registers until the end (lane groups added by two shuffles). Every Q fragment
+// read feeds the products of KS 16-key subtiles. Queries are split over
+// blocks (QC rows each) so that the causal triangle fills the chip evenly; a
+// second kernel adds the splits in a fixed order. No atomics.
+
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_cache.h"
+#include "kat_internal.h"
+
+namespace kat {
+
+using namespace mfma;
+
+struct KeywArgs {
+  const void* q;
+  const void* k;
+  const float* L;       // [B, H, T] by sl
+  float* out;           // [B, H, T] by so
+  const float* slopes;  // [H]
+  const uint8_t* mask;  // [B, T]: row b at mask + b * smask; or nullptr
+  int B, H, T, D;
+  int lo;               // first query that counts
+  int qc, chunks;       // queries per block; most chunks of a key block
+  int64_t sq[3], sk[3], sl[3], so[2], smask;
+  float scale, eps;
+  float* part;          // [chunks][B*H][T], or nullptr (one chunk)
+};
+
+constexpr int kKwWaves = 4;
+// a row in 16-bit units
+template <typename T, int W> constexpr int kw_units() { return W * (int)sizeof(T) / 2; }
+// 16-key subtiles per wave: their fragments take U / 8 registers each
+template <int U> constexpr int kw_ks() { return U <= 128 ? 4 : U == 256 ? 2 : 1; }
+// query rows per LDS tile
+template <int U> constexpr int kw_rows() { return U == 512 ? 32 : 64; }
+
+template <typename T, int W, bool KM>
+__global__ __launch_bounds__(64 * kKwWaves, (kw_units<T, W>() == 512 ? 1 : 2)) void attn_keyw_k(KeywArgs a) {
+  constexpr int ES = (int)sizeof(T), U = kw_units<T, W>(), KK = U / 32, KS = kw_ks<U>(), QR = kw_rows<U>();
+  constexpr int BK = 16 * KS * kKwWaves;  // keys per block
+  __shared__ short sq[2][QR * U];
+  __shared__ float sc[2][QR];  // 1 / (16 (L + eps)) of the tile's queries; 0: the query does not count
+
+  int bh, kb;
+  block_order((int)blockIdx.x, a.B * a.H, bh, kb);
+  const int b = bh / a.H, h = bh - b * a.H;
+  const int T_ = a.T;
+  const int r0 = std::max(a.lo, kb * BK) + (int)blockIdx.y * a.qc;
+  const int r1 = std::min(T_, r0 + a.qc);
+  if (r0 >= r1) return;  // fewer chunks than the longest key block has
+  const int lane = threadIdx.x & 63, w = wave_id();
+  const int g = lane >> 4, li = lane & 15;
+  const int kw = kb * BK + w * 16 * KS;  // the wave's first key
+
+  const char* qp = (const char*)((const T*)a.q + b * a.sq[0] + h * a.sq[1]);
+  const char* kp = (const char*)((const T*)a.k + b * a.sk[0] + h * a.sk[1]);
+  const int64_t sqb = a.sq[2] * ES, skb = a.sk[2] * ES;
+  const float* lp = a.L + b * a.sl[0] + h * a.sl[1];
+  const uint8_t* mp = KM ? a.mask + b * a.smask : nullptr;
+  const float slope = a.slopes[h], scale = a.scale;
+  const int cols = a.D * ES / 16;
+
+  TileDma<U, kKwWaves, QR> dq;
+  dq.init(w, lane, (uint32_t)(sqb / 2), a.D * ES / 2);
+  auto issue = [&](short* tile, int row) __attribute__((always_inline)) {
+    const int64_t left = (int64_t)(T_ - 1 - row) * sqb + a.D * ES;  // bytes from this row to the last one's end
+    dq.issue_rows(tile, qp + (int64_t)row * sqb, (uint32_t)std::min<int64_t>(left, 0x7fffffff), w);
+  };
+  auto cinv = [&](int row) __attribute__((always_inline)) {
+    const bool in = row < r1 && (!KM || mp[std::min(row, T_ - 1)] != 0);
+    const float l = lp[(int64_t)std::min(row, T_ - 1) * a.sl[2]];
+    return in ? 1.f / (16.f * (l + a.eps)) : 0.f;
+  };
+
+  issue(sq[0], r0);
+  i16x8 kf[KS][KK];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      const int p = 4 * kk + g;
+      kf[ks][kk] = i16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (p < cols)
+        kf[ks][kk] = *reinterpret_cast<const i16x8*>(kp + (int64_t)std::min(kw + 16 * ks + li, T_ - 1) * skb + 16 * p);
+    }
+  if (threadIdx.x < QR) sc[0][threadIdx.x] = cinv(r0 + (int)threadIdx.x);
+  float bl[4];  // slope (key - q) of a 16 x 16 piece: the lane's part
+#pragma unroll
+  for (int j = 0; j < 4; ++j) bl[j] = slope * (float)(li - 4 * g - j);
+  f32x4 acc[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) acc[ks] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // the tile's rows row .. row + QR - 1 against the wave's keys. MASKED: it
+  // touches the diagonal or holds a query that does not count (whose values may
+  // be anything)
+  auto tile = [&](auto masked_tag, int row, const short* qt, const float* ct) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(masked_tag)::value;
+#pragma unroll
+    for (int hr = 0; hr < QR; hr += 16) {
+      f32x4 s_[KS];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s_[ks] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const i16x8 qa = lds16(qt + soff<U>(hr + li, 32 * kk + 8 * g));
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s_[ks] = dot64<T>(qa, kf[ks][kk], s_[ks]);
+      }
+      const f32x4 c = *reinterpret_cast<const f32x4*>(ct + hr + 4 * g);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const float tterm = slope * (float)(kw + 16 * ks - row - hr);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float s = fmaf(s_[ks][j], scale, bl[j] + tterm);
+          const float r = __builtin_amdgcn_rcpf(fabsf(s) + 1.f);
+          const float t = fmaf(s, r, 1.f);
+          const float t2 = t * t;
+          const float f = t2 * t2;
+          if constexpr (MASKED) {
+            const bool in = c[j] != 0.f && kw + 16 * ks + li <= row + hr + 4 * g + j;
+            acc[ks][j] = fmaf(in ? f : 0.f, in ? c[j] : 0.f, acc[ks][j]);
+          } else {
+            acc[ks][j] = fmaf(f, c[j], acc[ks][j]);
+          }
+        }
+      }
+    }
+  };
+
+  dma_wait();
+  __syncthreads();
+  auto step = [&](int row, auto buf_tag) __attribute__((always_inline)) {
+    constexpr int buf = decltype(buf_tag)::value;
+    const bool more = row + QR < r1;
+    float cn = 0.f;
+    if (more) {
+      issue(sq[buf ^ 1], row + QR);
+      if (threadIdx.x < QR) cn = cinv(row + QR + (int)threadIdx.x);
+    }
+    if (row + QR - 1 >= kw) {  // else every key of the wave lies past the tile's queries
+      bool plain = row >= kw + 16 * KS - 1;
+      if constexpr (KM) plain = plain && __builtin_amdgcn_ballot_w64(lane < QR && sc[buf][lane % QR] == 0.f) == 0ull;
+      if (plain) tile(std::false_type{}, row, sq[buf], sc[buf]);
+      else tile(std::true_type{}, row, sq[buf], sc[buf]);
+    }
+    if (more && threadIdx.x < QR) sc[buf ^ 1][threadIdx.x] = cn;
+    dma_wait();
+    __syncthreads();
+  };
+  for (int row = r0; row < r1; row += 2 * QR) {
+    step(row, std::integral_constant<int, 0>{});
+    if (row + QR < r1) step(row + QR, std::integral_constant<int, 1>{});
+  }
+
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    float t = (acc[ks][0] + acc[ks][1]) + (acc[ks][2] + acc[ks][3]);
+    t += __shfl_xor(t, 16, 64);
+    t += __shfl_xor(t, 32, 64);
+    const int key = kw + 16 * ks + li;
+    if (g == 0 && key < T_) {
+      if (KM && mp[key] == 0) t = 0.f;
+      if (a.part) a.part[((int64_t)blockIdx.y * a.B * a.H + bh) * T_ + key] = t;
+      else a.out[b * a.so[0] + h * a.so[1] + key] = t;
+    }
+  }
+}
+
+// adds the chunks of each key in order
+__global__ __launch_bounds__(256) void attn_keyw_sum_k(KeywArgs a, int bk) {
+  const int bh = blockIdx.y, b = bh / a.H, h = bh - b * a.H;
+  const int key = blockIdx.x * 256 + threadIdx.x;
+  if (key >= a.T) return;
+  const int rows = a.T - std::max(a.lo, key / bk * bk);
+  const int nc = (rows + a.qc - 1) / a.qc;
+  const int64_t step = (int64_t)a.B * a.H * a.T;
+  const float* p = a.part + (int64_t)bh * a.T + key;
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
+  int c = 0;
+  for (; c + 4 <= nc; c += 4) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) t[r] += p[(c + r) * step];
+  }
+#pragma unroll
+  for (int r = 0; r < 3; ++r)
+    if (c + r < nc) t[r] += p[(c + r) * step];
+  a.out[b * a.so[0] + h * a.so[1] + key] = (t[0] + t[1]) + (t[2] + t[3]);
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+// layout widths: 64, 128, 256 (16-bit types: D a multiple of 8 up to 256), 32
+// .. 256 (fp32: multiples of 4 up to 256), the head dims of the MFMA forward
+static int keyw_layout(int64_t D, int dtype) {
+  if (dtype == KAT_F32 && D > 128 && D <= 256 && D % 4 == 0) return 256;
+  return cache_layout(D, dtype);
+}
+static int keyw_block_keys(int W, int dtype) {
+  const int U = W * dtype_size(dtype) / 2;
+  return 16 * kKwWaves * (U <= 128 ? 4 : U == 256 ? 2 : 1);
+}
+
+// queries per block: about four blocks per CU, whole 64-row tiles
+static void keyw_plan(int64_t B, int64_t H, int64_t T, int64_t lo, int W, int dtype, int& qc, int& chunks) {
+  const int64_t bk = keyw_block_keys(W, dtype);
+  int64_t rows = 0;  // (key block, query row) pairs of one head
+  for (int64_t k = 0; k < T; k += bk) rows += T - std::max(lo, k);
+  int64_t c = (rows * B * H + 4 * num_cus() - 1) / (4 * num_cus());
+  c = std::max<int64_t>(64, (c + 63) / 64 * 64);
+  chunks = (int)((T - lo + c - 1) / c);
+  qc = (int)std::min<int64_t>(c, 0x3fffffc0);
+}
+
+template <typename T, int W> static int launch_keyw(const KeywArgs& a, hipStream_t st) {
+  constexpr int U = kw_units<T, W>(), BK = 16 * kw_ks<U>() * kKwWaves;
+  const dim3 grid((unsigned)((a.T + BK - 1) / BK * a.B * a.H), (unsigned)a.chunks);
+  if (a.mask) hipLaunchKernelGGL((attn_keyw_k<T, W, true>), grid, dim3(64 * kKwWaves), 0, st, a);
+  else hipLaunchKernelGGL((attn_keyw_k<T, W, false>), grid, dim3(64 * kKwWaves), 0, st, a);
+  if (int rc = check_launch("kat_attn_key_weights")) return rc;
+  if (!a.part) return KAT_OK;
+  hipLaunchKernelGGL(attn_keyw_sum_k, dim3((unsigned)((a.T + 255) / 256), (unsigned)(a.B * a.H)), dim3(256), 0, st, a, BK);
+  return check_launch("kat_attn_key_weights (sum)");
+}
+template <typename T> static int keyw_w(const KeywArgs& a, int W, hipStream_t st) {
+  switch (W) {
+    case 32: if constexpr (sizeof(T) == 4) return launch_keyw<T, 32>(a, st); break;
+    case 64: return launch_keyw<T, 64>(a, st);
+    case 128: return launch_keyw<T, 128>(a, st);
+    case 256: return launch_keyw<T, 256>(a, st);
+  }
+  return fail(KAT_EUNSUPPORTED, "kat_attn_key_weights: head dim %d", a.D);
+}
+
+}  // namespace kat
+
+using namespace kat;
+
+extern "C" size_t kat_attn_key_weights_workspace_size(int64_t B, int64_t H, int64_t T, int64_t D, int64_t last,
+                                                      int dtype) {
+  const int W = keyw_layout(D, dtype);
+  if (B <= 0 || H <= 0 || T <= 0 || last < 0 || !W) return 0;
+  int qc, chunks;
+  keyw_plan(B, H, T, last == 0 ? 0 : std::max<int64_t>(0, T - last), W, dtype, qc, chunks);
+  return chunks == 1 ? 0 : (size_t)chunks * B * H * T * sizeof(float);
+}
+
+extern "C" int kat_attn_key_weights(const void* q, const void* k, const float* L, float* weights,
+                                    const float* slopes, const uint8_t* token_mask, int64_t mask_stride_b,
+                                    void* workspace, size_t workspace_bytes, int64_t B, int64_t H, int64_t T,
+                                    int64_t D, int64_t last, const int64_t* strides, float scale, float eps,
+                                    int dtype, void* stream) {
+  const char* nm = "kat_attn_key_weights";
+  if (B < 0 || H < 0 || T < 0 || D < 0 || last < 0) return fail(KAT_EINVAL, "%s: negative size", nm);
+  if (B > 0xffff || H > 0xffff || B * H > 0xffff || T > 0x3fffff)
+    return fail(KAT_EUNSUPPORTED, "%s: B*H or T too large", nm);
+  const int W = keyw_layout(D, dtype);
+  if (!W) return fail(KAT_EUNSUPPORTED, "%s: head dim %lld with dtype %d", nm, (long long)D, dtype);
+  if (B * H * T == 0) return KAT_OK;
+  if (!q || !k || !L || !weights || !slopes || !strides) return fail(KAT_EINVAL, "%s: null pointer", nm);
+  const int esz = dtype_size(dtype);
+  for (int t = 0; t < 6; ++t)
+    if ((strides[t] * esz) % 16 != 0) return fail(KAT_EUNSUPPORTED, "%s: strides must keep rows 16-byte aligned", nm);
+  if (!aligned16(q) || !aligned16(k)) return fail(KAT_EUNSUPPORTED, "%s: tensors must be 16-byte aligned", nm);
+  if (T > 1 && (strides[2] < D || strides[5] < D)) return fail(KAT_EINVAL, "%s: row stride < D", nm);
+  // a tile's rows are addressed by 31-bit byte offsets
+  if (T > 1 && strides[2] * esz * 64 > 0x7fffffff) return fail(KAT_EUNSUPPORTED, "%s: q row stride too large", nm);
+  KeywArgs a = {};
+  a.q = q;
+  a.k = k;
+  a.L = L;
+  a.out = weights;
+  a.slopes = slopes;
+  a.mask = token_mask;
+  a.smask = mask_stride_b;
+  a.B = (int)B;
+  a.H = (int)H;
+  a.T = (int)T;
+  a.D = (int)D;
+  a.lo = last == 0 ? 0 : (int)std::max<int64_t>(0, T - last);
+  for (int i = 0; i < 3; ++i) {
+    a.sq[i] = strides[i];
+    a.sk[i] = strides[3 + i];
+    a.sl[i] = strides[6 + i];
+  }
+  if (T == 1) a.sq[2] = D;  // one row: its stride may be anything
+  a.so[0] = strides[9];
+  a.so[1] = strides[10];
+  a.scale = scale;
+  a.eps = eps;
+  keyw_plan(B, H, T, a.lo, W, dtype, a.qc, a.chunks);
+  const size_t need = kat_attn_key_weights_workspace_size(B, H, T, D, last, dtype);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(KAT_EINVAL, "%s: workspace %zu bytes < required %zu", nm, workspace_bytes, need);
+  a.part = need ? (float*)workspace : nullptr;
+  if (a.chunks > 0xffff || (T + 63) / 64 * B * H > 0x7fffffff) return fail(KAT_EUNSUPPORTED, "%s: B*H*T too large", nm);
+  const hipStream_t st = as_stream(stream);
+  switch (dtype) {
+    case KAT_F32: return keyw_w<float>(a, W, st);
+    case KAT_BF16: return keyw_w<bf16>(a, W, st);
+    case KAT_F16: return keyw_w<f16>(a, W, st);
+  }
+  return fail(KAT_EUNSUPPORTED, "%s: unsupported dtype %d", nm, dtype);
+}

@@ -271,6 +271,14 @@ template <int D, int NW, int ROWS = 64> struct TileDma {
 #pragma unroll
     for (int u = 0; u < SEGS; ++u) dma16<NT>(r, l0 + (uint32_t)(u * RPS * D * 2), off[u]);
   }
+  // the tile whose first row is at first, of a matrix that ends `bytes` after it
+  // (the caller adds the row offset in 64 bits)
+  __device__ __forceinline__ void issue_rows(short* tile, const void* first, uint32_t bytes, int w) const {
+    const i32x4 r = rsrc_words(first, bytes);
+    const uint32_t l0 = lds_addr(tile) + (uint32_t)(__builtin_amdgcn_readfirstlane(w) * SEGS * RPS * D * 2);
+#pragma unroll
+    for (int u = 0; u < SEGS; ++u) dma16(r, l0 + (uint32_t)(u * RPS * D * 2), off[u]);
+  }
 };
 
 // Block order. Workgroups are dispatched round-robin over the 8 XCDs (block id

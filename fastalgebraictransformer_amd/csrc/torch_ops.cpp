@@ -18,6 +18,7 @@
 // examined again there.
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -628,6 +629,155 @@ std::optional<std::tuple<Tensor, Tensor>> decode(const Tensor& q, const Tensor& 
   return std::make_tuple(out, L);
 }
 
+// ---------------------------------------------------------------------------
+// operators over a cache (kv_cache.py states their arguments); no gradients
+// ---------------------------------------------------------------------------
+
+// a plain int32 tensor on q's device
+bool ints(const Tensor& q, const Tensor& t) {
+  return t.defined() && t.is_cuda() && t.device() == q.device() && t.layout() == at::kStrided &&
+         t.scalar_type() == at::kInt && !t.key_set().has(c10::DispatchKey::Python);
+}
+// [B] int32, or none
+bool lengths_ok(const Tensor& q, const std::optional<Tensor>& n, int64_t B) {
+  return !n || (ints(q, *n) && n->is_contiguous() && n->numel() == B);
+}
+// [B, H, T] with unit t-stride
+bool rows_ok(const Tensor& t, int64_t B, int64_t H, int64_t T) {
+  return t.dim() == 3 && t.size(0) == B && t.size(1) == H && t.size(2) == T && (T <= 1 || t.stride(2) == 1);
+}
+bool positions_ok(const Tensor& q, const std::optional<Tensor>& p, int64_t B, int64_t H, int64_t T) {
+  return !p || (ints(q, *p) && rows_ok(*p, B, H, T));
+}
+// a dim's writers must not meet
+bool apart(const Tensor& t) {
+  for (int64_t d = 0; d + 1 < t.dim(); ++d)
+    if (t.size(d) > 1 && t.stride(d) < t.size(-1)) return false;
+  return true;
+}
+// q (its last dim D), caches k, v [B, H, T, D] of one dtype, slopes [H]
+bool cache_ok(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& slopes) {
+  return untraced() && attn_dtype(q) && same_place(q, {&k, &v}) && k.scalar_type() == q.scalar_type() &&
+         v.scalar_type() == q.scalar_type() && k.dim() == 4 && k.sizes() == v.sizes() && k.size(0) == q.size(0) &&
+         k.size(1) == q.size(1) && k.size(3) == q.size(-1) && q.numel() != 0 && k.numel() != 0 &&
+         q.stride(-1) == 1 && k.stride(3) == 1 && v.stride(3) == 1 &&
+         (slopes_ok(q, slopes, q.size(1)) || slopes_narrow(q, slopes, q.size(1)));
+}
+
+// q [B, H, N, D], parents [B, N] or [N]: (out, L)
+std::optional<std::tuple<Tensor, Tensor>> tree(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& slopes,
+                                               double scale, const Tensor& parents,
+                                               const std::optional<Tensor>& lengths,
+                                               const std::optional<Tensor>& positions, double eps) {
+  if (q.dim() != 4 || !cache_ok(q, k, v, slopes)) return std::nullopt;
+  const int64_t B = q.size(0), H = q.size(1), N = q.size(2), D = q.size(3), T = k.size(2);
+  if (!ints(q, parents) || parents.dim() < 1 || parents.dim() > 2 || parents.size(-1) != N ||
+      (parents.dim() == 2 && parents.size(0) != B) || (N > 1 && parents.stride(-1) != 1) ||
+      !lengths_ok(q, lengths, B) || !positions_ok(q, positions, B, H, T))
+    return std::nullopt;
+  at::NoGradGuard g;
+  const c10::DeviceGuard dg(q.device());
+  const Tensor sl = slopes_of(slopes);
+  // the output's layout follows the query's: token-major where that is
+  const bool tm = q.stride(1) < q.stride(2);
+  Tensor out = at::empty(tm ? at::IntArrayRef({B, N, H, D}) : at::IntArrayRef({B, H, N, D}),
+                         q.options().memory_format(at::MemoryFormat::Contiguous));
+  if (tm) out = out.transpose(1, 2);
+  Tensor L = at::empty({B, H, N}, q.options().dtype(at::kFloat));
+  const size_t wsb = kat_attn_tree_workspace_size(B, H, N, T, D, code(q));
+  const Tensor ws = wsb ? bytes(wsb, q) : Tensor();
+  const int64_t s[12] = {q.stride(0), q.stride(1), q.stride(2), k.stride(0), k.stride(1), k.stride(2),
+                         v.stride(0), v.stride(1), v.stride(2), out.stride(0), out.stride(1), out.stride(2)};
+  int64_t ps[2] = {0, 0};
+  if (positions) {
+    ps[0] = positions->stride(0);
+    ps[1] = positions->stride(1);
+  }
+  check(kat_attn_tree(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), L.data_ptr<float>(),
+                      sl.data_ptr<float>(), parents.data_ptr<int32_t>(), parents.dim() == 2 ? parents.stride(0) : 0,
+                      lengths ? lengths->data_ptr<int32_t>() : nullptr,
+                      positions ? positions->data_ptr<int32_t>() : nullptr, ps, wsb ? ws.data_ptr() : nullptr, wsb, B,
+                      H, N, T, D, s, (float)scale, (float)eps, code(q), stream(q)),
+        "kat_attn_tree");
+  return std::make_tuple(out, L);
+}
+
+// q [B, H, D], weights [B, H, T] updated in place: (out, L)
+std::optional<std::tuple<Tensor, Tensor>> decode_accumulate(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                            const Tensor& slopes, double scale, const Tensor& weights,
+                                                            const std::optional<Tensor>& lengths,
+                                                            const std::optional<Tensor>& positions, double eps) {
+  if (q.dim() != 3 || !cache_ok(q, k, v, slopes)) return std::nullopt;
+  const int64_t B = q.size(0), H = q.size(1), D = q.size(2), T = k.size(2);
+  if (!same_place(q, {&weights}) || weights.scalar_type() != at::kFloat || !rows_ok(weights, B, H, T) ||
+      !apart(weights) || !lengths_ok(q, lengths, B) || !positions_ok(q, positions, B, H, T))
+    return std::nullopt;
+  at::NoGradGuard g;
+  const c10::DeviceGuard dg(q.device());
+  const Tensor sl = slopes_of(slopes);
+  Tensor out = at::empty({B, H, D}, q.options().memory_format(at::MemoryFormat::Contiguous));
+  Tensor L = at::empty({B, H}, q.options().dtype(at::kFloat));
+  const size_t wsb = kat_attn_decode_accum_workspace_size(B, H, T, D, code(q));
+  const Tensor ws = bytes(wsb, q);
+  const int64_t s[10] = {q.stride(0), q.stride(1), k.stride(0), k.stride(1), k.stride(2),
+                         v.stride(0), v.stride(1), v.stride(2), out.stride(0), out.stride(1)};
+  const int64_t wp[4] = {weights.stride(0), weights.stride(1), positions ? positions->stride(0) : 0,
+                         positions ? positions->stride(1) : 0};
+  check(kat_attn_decode_accum(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), L.data_ptr<float>(),
+                              sl.data_ptr<float>(), weights.data_ptr<float>(),
+                              lengths ? lengths->data_ptr<int32_t>() : nullptr,
+                              positions ? positions->data_ptr<int32_t>() : nullptr, wp, ws.data_ptr(), wsb, B, H, T, D,
+                              s, (float)scale, (float)eps, code(q), stream(q)),
+        "kat_attn_decode_accum");
+  return std::make_tuple(out, L);
+}
+
+// q, k [B, H, T, D], L [B, H, T]: weights [B, H, T]; last == 0: every query
+std::optional<Tensor> key_weights(const Tensor& q, const Tensor& k, const Tensor& slopes, double scale, const Tensor& L,
+                                  const std::optional<Tensor>& km, int64_t last, double eps) {
+  if (q.dim() != 4 || !cache_ok(q, k, k, slopes) || k.sizes() != q.sizes()) return std::nullopt;
+  const int64_t B = q.size(0), H = q.size(1), T = q.size(2), D = q.size(3);
+  if (!same_place(q, {&L}) || L.scalar_type() != at::kFloat || L.dim() != 3 || L.sizes() != q.sizes().slice(0, 3) ||
+      !mask_ok(q, km, B, T))
+    return std::nullopt;
+  at::NoGradGuard g;
+  const c10::DeviceGuard dg(q.device());
+  const Tensor sl = slopes_of(slopes), mask = mask_of(km).t;
+  Tensor w = at::empty({B, H, T}, q.options().dtype(at::kFloat));
+  const size_t wsb = kat_attn_key_weights_workspace_size(B, H, T, D, last, code(q));
+  const Tensor ws = wsb ? bytes(wsb, q) : Tensor();
+  const int64_t s[11] = {q.stride(0), q.stride(1), q.stride(2), k.stride(0), k.stride(1), k.stride(2),
+                         L.stride(0), L.stride(1), L.stride(2), w.stride(0), w.stride(1)};
+  check(kat_attn_key_weights(q.data_ptr(), k.data_ptr(), L.data_ptr<float>(), w.data_ptr<float>(),
+                             sl.data_ptr<float>(), mask.defined() ? mask.data_ptr<uint8_t>() : nullptr, T,
+                             wsb ? ws.data_ptr() : nullptr, wsb, B, H, T, D, last, s, (float)scale, (float)eps,
+                             code(q), stream(q)),
+        "kat_attn_key_weights");
+  return w;
+}
+
+// caches of one layout; the outputs are the inputs (in place) or other tensors.
+// The wrapper has checked shapes and types.
+void evict(const Tensor& k, const Tensor& v, const Tensor& w, const Tensor& p, const std::optional<Tensor>& n,
+           const Tensor& ko, const Tensor& vo, const Tensor& wo, const Tensor& po, const Tensor& no, int64_t keep,
+           int64_t recent, bool in_place) {
+  const c10::DeviceGuard dg(k.device());
+  const int64_t B = k.size(0), H = k.size(1), T = k.size(2), D = k.size(3);
+  const size_t wsb = kat_kv_evict_workspace_size(B, H, keep);
+  const Tensor ws = bytes(wsb, k);
+  int64_t s[20];
+  int i = 0;
+  for (const Tensor* t : {&k, &v, &ko, &vo})
+    for (int d = 0; d < 3; ++d) s[i++] = t->stride(d);
+  for (const Tensor* t : {&w, &p, &wo, &po})
+    for (int d = 0; d < 2; ++d) s[i++] = t->stride(d);
+  check(kat_kv_evict(k.data_ptr(), v.data_ptr(), w.data_ptr<float>(), p.data_ptr<int32_t>(),
+                     n ? n->data_ptr<int32_t>() : nullptr, ko.data_ptr(), vo.data_ptr(), wo.data_ptr<float>(),
+                     po.data_ptr<int32_t>(), no.data_ptr<int32_t>(), ws.data_ptr(), wsb, B, H, T, D, keep, recent,
+                     in_place, s, code(k), stream(k)),
+        "kat_kv_evict");
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_katops, m) {
@@ -642,6 +792,10 @@ PYBIND11_MODULE(_katops, m) {
   m.def("attention_masked", &attention_masked, nogil());
   m.def("attention_packed", &attention_packed, nogil());
   m.def("decode", &decode, nogil());
+  m.def("tree", &tree, nogil());
+  m.def("decode_accumulate", &decode_accumulate, nogil());
+  m.def("key_weights", &key_weights, nogil());
+  m.def("evict", &evict, nogil());
   // the layout rules alone (any device): (in place?, rows, cols, row stride)
   // of rows2d, and whether [B, H, T, D] operands lie in the MFMA envelope
   m.def("rows2d", [](const Tensor& t) {

@@ -281,6 +281,88 @@ int kat_attn_decode_noalloc(const void* q, const void* k, const void* v, void* o
                             int dtype, void* stream);
 
 /* ----------------------------------------------------------------------
+ * Attention of a tree of drafted tokens over a KV cache (one pass of
+ * speculative decoding); no counterpart in the reference. With n = lengths[b]
+ * (T when lengths is NULL, at most T), the last N of the n cached rows hold the
+ * drafted tokens' keys and values, token i in row c + i, c = n - N. parents
+ * [B, N] (row b at parents + b * parents_stride_b; 0: one tree for all) gives
+ * the token that i hangs on, parents[i] < i, or -1 for the context; any other
+ * value marks an absent token, as is every token below one. Token i attends to
+ * rows 0 .. c - 1 and to the rows of itself and its ancestors:
+ *   s = scale <q_i, k_j> - slope_h (p_i - p_j),  f = sigma(s)^4
+ *   L_i = sum f (fp32, without eps),  out_i = sum f v_j / (L_i + eps)
+ * Positions p: the row (context), c + the token's depth (tokens); or, with
+ * positions (int32 [B, H, T], (b, h) strides in pos_strides, unit t-stride),
+ * positions[row]. Absent tokens, and all tokens of a row with n < N, get out =
+ * 0, L = 0. A row that a token does not attend to may hold anything, NaN
+ * included; rows at or past n are not read. N <= 64; N = 1 is kat_attn_decode.
+ * q, out: [B, H, N, D], k, v: [B, H, T, D]; strides: 12 int64 = (b, h, row) of
+ * q, k, v, out, unit d-stride, 16-byte aligned rows. L: [B*H*N] or NULL. Types
+ * and head dims as kat_attn_decode. Deterministic. The workspace may be NULL
+ * where its size is 0. */
+size_t kat_attn_tree_workspace_size(int64_t B, int64_t H, int64_t N, int64_t T, int64_t D, int dtype);
+int kat_attn_tree(const void* q, const void* k, const void* v, void* out, float* L,
+                  const float* slopes, const int32_t* parents, int64_t parents_stride_b,
+                  const int32_t* lengths, const int32_t* positions, const int64_t* pos_strides,
+                  void* workspace, size_t workspace_bytes, int64_t B, int64_t H, int64_t N,
+                  int64_t T, int64_t D, const int64_t* strides, float scale, float eps, int dtype,
+                  void* stream);
+
+/* kat_attn_decode that also adds each row's attention weight to its running
+ * total: weights[b, h, j] += f_j / (L + eps) for j < n (fp32, in place; totals
+ * at or past n are left as they are). With positions (int32 [B, H, T]) the
+ * distance of row j is positions[n - 1] - positions[j] instead of n - 1 - j: a
+ * cache whose rows have been evicted. wp_strides: 4 int64 = (b, h) of weights
+ * and of positions, unit t-stride; weights must not overlap themselves. Other
+ * arguments as kat_attn_decode. No counterpart in the reference. */
+size_t kat_attn_decode_accum_workspace_size(int64_t B, int64_t H, int64_t T, int64_t D, int dtype);
+int kat_attn_decode_accum(const void* q, const void* k, const void* v, void* out, float* L,
+                          const float* slopes, float* weights, const int32_t* lengths,
+                          const int32_t* positions, const int64_t* wp_strides, void* workspace,
+                          size_t workspace_bytes, int64_t B, int64_t H, int64_t T, int64_t D,
+                          const int64_t* strides, float scale, float eps, int dtype, void* stream);
+
+/* The attention weight each key of a prompt receives from its queries:
+ *   weights[b, h, j] = sum_i f_ij / (L_i + eps),  i >= j
+ * with f as kat_attn_fwd and L the row sums it stored. last > 0: only the last
+ * `last` queries count. token_mask (uint8 [B, T], or NULL): a dropped token
+ * neither gives nor receives weight, whatever its q, k and L hold (L then
+ * comes from kat_attn_fwd_masked with the same mask). strides: 11 int64 = (b, h,
+ * t) of q, k and L and (b, h) of weights (unit t-stride). Types and head dims:
+ * those of the MFMA forward (KAT_BF16 / KAT_F16 multiples of 8, KAT_F32
+ * multiples of 4, up to 256), 16-byte aligned rows. Deterministic; the workspace
+ * may be NULL where its size is 0. No counterpart in the reference. */
+size_t kat_attn_key_weights_workspace_size(int64_t B, int64_t H, int64_t T, int64_t D, int64_t last,
+                                           int dtype);
+int kat_attn_key_weights(const void* q, const void* k, const float* L, float* weights,
+                         const float* slopes, const uint8_t* token_mask, int64_t mask_stride_b,
+                         void* workspace, size_t workspace_bytes, int64_t B, int64_t H, int64_t T,
+                         int64_t D, int64_t last, const int64_t* strides, float scale, float eps,
+                         int dtype, void* stream);
+
+/* Eviction from a KV cache by accumulated weight; no counterpart in the
+ * reference. Of the n = lengths[b] filled rows (T when lengths is NULL, clamped
+ * to [0, T]) of each (b, h), m = min(n, keep) stay: first those with a position
+ * above positions[n - 1] - recent, then those with the largest weights, ties to
+ * the lower row; a NaN weight ranks above every number. lengths_out[b] (may be
+ * NULL) becomes m.
+ *   in_place == 0: the kept rows of k, v, weights, positions go to rows 0 .. m - 1
+ *     of the outputs (at least min(T, keep) rows each), in their order; the
+ *     outputs must not overlap the inputs, and rows at or past m are left alone.
+ *   in_place != 0: the outputs are the inputs; kept rows below m stay, the kept
+ *     rows at or past m move, in order, into the given-up rows below m.
+ * k, v: [B, H, T, D] of dtype, any head dim of whole 16-byte pieces, 16-byte
+ * aligned rows; weights fp32 and positions int32 [B, H, T], unit t-stride.
+ * strides: 20 int64 = (b, h, t) of k, v, k_out, v_out, then (b, h) of weights,
+ * positions, weights_out, positions_out. recent <= keep. */
+size_t kat_kv_evict_workspace_size(int64_t B, int64_t H, int64_t keep);
+int kat_kv_evict(const void* k, const void* v, const float* weights, const int32_t* positions,
+                 const int32_t* lengths, void* k_out, void* v_out, float* weights_out,
+                 int32_t* positions_out, int32_t* lengths_out, void* workspace,
+                 size_t workspace_bytes, int64_t B, int64_t H, int64_t T, int64_t D, int64_t keep,
+                 int64_t recent, int in_place, const int64_t* strides, int dtype, void* stream);
+
+/* ----------------------------------------------------------------------
  * Measurement helper (no counterpart in the reference; used by bench.py to
  * report a measured MFMA rate beside the spec peak). `blocks` x 256 threads
  * each run `iters` rounds of 16 independent v_mfma_f32_16x16x32_bf16 chains
