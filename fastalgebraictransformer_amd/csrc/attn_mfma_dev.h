@@ -188,7 +188,18 @@ __device__ __forceinline__ void dma16(const i32x4& r, uint32_t lds, uint32_t vof
                  "s"(r)
                  : "memory");
 }
+// the same for 4 bytes per lane, into LDS at lds + 4 l
+__device__ __forceinline__ void dma4(const i32x4& r, uint32_t lds, uint32_t voff) {
+  const uint32_t la = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(la), "v"(voff), "s"(r) : "memory");
+}
 __device__ __forceinline__ void dma_wait() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+// all but the N youngest vector-memory operations of the wave are complete
+// (vmcnt's low four bits are bits 3..0 of the encoding, its high two 15..14)
+template <int N> __device__ __forceinline__ void dma_wait_but() {
+  static_assert(N >= 0 && N < 64, "vmcnt has six bits");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+}
 
 // ---------------------------------------------------------------------------
 // LDS tiles: rows of D 16-bit elements with the 16-byte chunks of row r XOR-ed
@@ -273,11 +284,12 @@ template <int D, int NW, int ROWS = 64> struct TileDma {
   }
   // the tile whose first row is at first, of a matrix that ends `bytes` after it
   // (the caller adds the row offset in 64 bits)
+  template <bool NT = false>
   __device__ __forceinline__ void issue_rows(short* tile, const void* first, uint32_t bytes, int w) const {
     const i32x4 r = rsrc_words(first, bytes);
     const uint32_t l0 = lds_addr(tile) + (uint32_t)(__builtin_amdgcn_readfirstlane(w) * SEGS * RPS * D * 2);
 #pragma unroll
-    for (int u = 0; u < SEGS; ++u) dma16(r, l0 + (uint32_t)(u * RPS * D * 2), off[u]);
+    for (int u = 0; u < SEGS; ++u) dma16<NT>(r, l0 + (uint32_t)(u * RPS * D * 2), off[u]);
   }
 };
 

@@ -17,17 +17,21 @@
 // bounds the call: 2 D dtype bytes and 4 N D flops per row, N = 64 in bf16 64
 // flops per byte against the card's ~230. As in the decode, the rows are split
 // into chunks, one block each, and sigma^4 needs no running maximum: blocks
-// write plain sums and a second kernel adds them in a fixed order. Inside a block
-// every wave takes row groups of its own (32 rows; 16 in fp32) for all queries,
-// so K and V pass through no shared tile and the loop has no barrier:
-//   S^T[row][q] = K Q^T    A = K straight from memory to registers (lane (g,
-//                          li) loads 16 bytes of row li), B = Q^T (registers)
+// write plain sums and a second kernel adds them in a fixed order.
+//
+// A block streams its rows through LDS in tiles of 64 (LDS-DMA, a ring of
+// NS stages, non-temporal: each row is used once), so rows in flight hold no
+// registers. Its four waves form QG query groups of 16 queries and KG = 4 / QG
+// row groups of a tile:
+//   S^T[row][q] = K Q^T    A = K (LDS rows)             B = Q^T (registers)
 //   f of S^T               lane (g, li) holds rows 4 g + j, query li
-//   O^T[d][q] += V^T f^T   A = V^T: the wave's rows go through an LDS tile of
-//                          its own and come back transposed; B = f packed to
-//                          the dtype (as the forward does), or fp32
-// The next group's rows are loaded before the current group is worked on.
-// Only groups that reach the tokens' rows (at most three) look at the ancestor
+//   O^T[d][q] += V^T f^T   A = V^T (LDS, transposed reads)  B = f packed to the
+//                          dtype as the forward does, or fp32
+// A first version gave every wave whole rows for all queries, loaded straight
+// into registers: at 64 queries the accumulators and fragments (192 registers)
+// left no room for the rows in flight, and it spilled (578 us at B=8, H=16, N=64,
+// T=8192, D=128, bf16).
+// Only tiles that reach the tokens' rows (two or three) look at the ancestor
 // masks, which each block derives from the parents by pointer doubling, one
 // lane per token.
 
@@ -61,26 +65,28 @@ struct TreeArgs {
 
 constexpr int kTreeMax = 64;  // tokens: one ancestor mask is one 64-bit word
 constexpr int kTreeWaves = 4;
+constexpr int kTreeRows = 64;  // rows of a tile
 
-// rows of one wave's group
-template <typename T> constexpr int tree_group() { return sizeof(T) == 2 ? 32 : 16; }
+// stages of the ring by a row's 16-bit units: two blocks per CU share 160 KB of
+// LDS up to U = 128 (a stage is 256 U bytes), one at U = 256
+template <int U> constexpr int tree_stages() { return U <= 64 ? 4 : 2; }
 
-template <typename T, int W, int QT, bool POS>
-__global__ __launch_bounds__(64 * kTreeWaves, QT == 4 || W == 256 ? 1 : 2) void attn_tree_k(TreeArgs a) {
+template <typename T, int W, int QG, bool POS>
+__global__ __launch_bounds__(64 * kTreeWaves, (W * (int)sizeof(T) > 256 ? 1 : 2)) void attn_tree_k(TreeArgs a) {
   constexpr int ES = (int)sizeof(T);
-  constexpr int RB = W * ES;             // bytes of a row
-  constexpr int KK = RB / 64;            // 64-byte column blocks
-  constexpr int G = tree_group<T>();     // rows of a group
-  constexpr int HH = G / 16;             // 16-row halves
-  constexpr int CPR = RB / 16;           // 16-byte pieces of a row
-  constexpr int NV = G * CPR / 64;       // V pieces per lane
-  constexpr int RPL = 64 / CPR;          // V rows per load instruction
+  constexpr int U = W * ES / 2;          // a row in 16-bit units, the unit of the tile helpers
+  constexpr int KK = U / 32;             // 64-byte column blocks
   constexpr int DS = W / 16;             // 16-wide d subtiles
-  constexpr int U = RB / 2;              // a row in 16-bit units, the unit of the tile helpers
-  static_assert(CPR <= 64 && NV >= 1, "row layout");
-  __shared__ short sv[kTreeWaves][G * U];
-  __shared__ f32x4 sx[kTreeWaves * DS * 64];  // the waves' sums of one query subtile
-  __shared__ float sl[kTreeWaves][16 * QT];
+  constexpr int TR = kTreeRows, NS = tree_stages<U>();
+  constexpr int KG = kTreeWaves / QG;    // row groups of a tile
+  constexpr int TK = TR / KG;            // rows of a wave's group
+  typedef TileDma<U, kTreeWaves, TR> Dma;
+  constexpr int OPS = 2 * Dma::SEGS + (POS ? 1 : 0);  // a wave's DMA operations per tile
+  constexpr int RING = NS * 2 * TR * U;
+  static_assert(RING * 2 >= kTreeWaves * DS * 1024, "the ring holds the waves' sums");
+  __shared__ __align__(16) short ring[RING];
+  __shared__ int spos[POS ? NS : 1][kTreeWaves][TR];
+  __shared__ float sl[kTreeWaves][16];
   __shared__ uint64_t sanc[kTreeMax];  // ancestors of token i, itself included; 0 if absent
   __shared__ int sdep[kTreeMax];       // depth of token i below the context
 
@@ -88,11 +94,39 @@ __global__ __launch_bounds__(64 * kTreeWaves, QT == 4 || W == 256 ? 1 : 2) void 
   const int split = blockIdx.x;
   const int lane = threadIdx.x & 63, w = wave_id();
   const int g = lane >> 4, li = lane & 15;
+  const int qg = w % QG, kg = w / QG;
   const int N = a.N;
   int n = a.lengths ? a.lengths[b] : a.T;
   n = min(n, a.T);
   const int c = n - N;       // rows of the context
   if (c < 0) n = 0;          // no room for the tokens: the row holds no draft
+
+  const char* kp = (const char*)((const T*)a.k + b * a.sk[0] + h * a.sk[1]);
+  const char* vp = (const char*)((const T*)a.v + b * a.sv[0] + h * a.sv[1]);
+  const int64_t skb = a.sk[2] * ES, svb = a.sv[2] * ES;
+  const int32_t* pp = POS ? a.positions + b * a.spos[0] + h * a.spos[1] : nullptr;
+
+  // this split's tiles
+  const int nt = (n + TR - 1) / TR;
+  const int per = (nt + a.splits - 1) / a.splits;
+  const int t0 = split * per, t1 = min(t0 + per, nt);
+
+  Dma dk, dv;
+  dk.init(w, lane, (uint32_t)(skb / 2), a.D * ES / 2);
+  dv.init(w, lane, (uint32_t)(svb / 2), a.D * ES / 2);
+  // rows past the last filled one, and columns past the head dim, read as zeros
+  auto issue = [&](int t) __attribute__((always_inline)) {
+    const int row = t * TR, st = (t - t0) % NS;
+    short* const kt = ring + st * 2 * TR * U;
+    const int64_t left = (int64_t)(n - 1 - row), lim = 0x7fffffff;
+    dk.template issue_rows<true>(kt, kp + row * skb, (uint32_t)min(left * skb + a.D * ES, lim), w);
+    dv.template issue_rows<true>(kt + TR * U, vp + row * svb, (uint32_t)min(left * svb + a.D * ES, lim), w);
+    if constexpr (POS)
+      dma4(rsrc_words(pp + row, (uint32_t)min(left + 1, (int64_t)TR) * 4), lds_addr(&spos[st][w][0]), (uint32_t)lane * 4);
+  };
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i)
+    if (t0 + i < t1) issue(t0 + i);
 
   if (w == 0) {
     // pointer doubling: after step i, anc holds the 2^i nearest ancestors and
@@ -118,227 +152,181 @@ __global__ __launch_bounds__(64 * kTreeWaves, QT == 4 || W == 256 ? 1 : 2) void 
   }
 
   const float slope = a.slopes[h], scale = a.scale;
-  const char* kp = (const char*)((const T*)a.k + b * a.sk[0] + h * a.sk[1]);
-  const char* vp = (const char*)((const T*)a.v + b * a.sv[0] + h * a.sv[1]);
-  const int64_t skb = a.sk[2] * ES, svb = a.sv[2] * ES;
-  const int32_t* pp = POS ? a.positions + b * a.spos[0] + h * a.spos[1] : nullptr;
-  const int cols = a.D * ES / 16;  // pieces of a row that hold columns
-
-  // this split's groups, dealt to the waves in turn
-  const int ng = (n + G - 1) / G;
-  const int per = (ng + a.splits - 1) / a.splits;
-  const int g0 = split * per, g1 = min(g0 + per, ng);
-
-  // pieces at or past the head dim re-read the row's first one (the query is
-  // zero there, and their output columns are not stored); rows past the last
-  // filled one re-read it
-  i16x8 kr[HH][KK], vr[NV];
-  auto load = [&](int gi) __attribute__((always_inline)) {
+  const int cols = a.D * ES / 16;  // 16-byte pieces of a row that hold columns
+  const int qi = 16 * qg + li;     // the lane's token
+  i16x8 qf[KK];
 #pragma unroll
-    for (int hh = 0; hh < HH; ++hh) {
-      const char* row = kp + (int64_t)min(gi * G + 16 * hh + li, n - 1) * skb;
+  for (int kk = 0; kk < KK; ++kk) {
+    const int p = 4 * kk + g;
+    qf[kk] = i16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    if (qi < N && p < cols)
+      qf[kk] = *reinterpret_cast<const i16x8*>((const char*)((const T*)a.q + b * a.sq[0] + h * a.sq[1] + qi * a.sq[2]) +
+                                               16 * p);
+  }
+  __syncthreads();  // masks and depths
+  const uint64_t anc = qi < N ? sanc[qi] : 0ull;
+  int qpos = 0;
+  if (qi < N && n > 0) qpos = POS ? pp[c + qi] : c + sdep[qi];
+
+  f32x4 oacc[DS];
+  float lsum = 0.f;
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) kr[hh][kk] = ld_piece_nt(row + 16 * (4 * kk + g < cols ? 4 * kk + g : 0));
+  for (int ds = 0; ds < DS; ++ds) oacc[ds] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // 16 rows at tile row hr (row k0 + hr of the cache) against the wave's
+  // queries: f of S^T. TAIL: the tile reaches the tokens' rows or the end
+  auto scores = [&](auto tail_tag, int k0, int hr, const short* kt, const int* pt) __attribute__((always_inline)) {
+    constexpr bool TAIL = decltype(tail_tag)::value;
+    f32x4 f = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) f = dot64<T>(lds16(kt + soff<U>(hr + li, 32 * kk + 8 * g)), qf[kk], f);
+    i32x4 kpos;
+    if constexpr (POS) kpos = *reinterpret_cast<const i32x4*>(pt + hr + 4 * g);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = k0 + hr + 4 * g + j;
+      const int tok = row - c;  // the drafted token in this row, if >= 0
+      int kp_ = row;
+      if constexpr (POS) kp_ = kpos[j];
+      else if constexpr (TAIL) kp_ = tok < 0 ? row : c + sdep[min(tok, kTreeMax - 1)];
+      const float s = fmaf(f[j], scale, -slope * (float)(qpos - kp_));
+      float x = sig2_pow4(s);
+      if constexpr (TAIL) {
+        const bool seen = tok < 0 ? anc != 0ull : tok < N && ((anc >> (tok & 63)) & 1ull);
+        x = seen ? x : 0.f;
+      }
+      f[j] = x;
     }
+    lsum += (f[0] + f[1]) + (f[2] + f[3]);
+    return f;
+  };
+  // O^T += V^T f^T over RN rows (16 or 32) at tile row hr
+  auto product = [&](auto rn_tag, int hr, const f32x4& x, const f32x4& y, const short* vt) __attribute__((always_inline)) {
+    constexpr int RN = decltype(rn_tag)::value;
+    if constexpr (ES == 4) {
 #pragma unroll
-    for (int u = 0; u < NV; ++u) {
-      const int r = u * RPL + lane / CPR, p = lane % CPR;
-      vr[u] = ld_piece_nt(vp + (int64_t)min(gi * G + r, n - 1) * svb + 16 * (p < cols ? p : 0));
+      for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+        for (int i = 0; i < RN / 16; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            oacc[ds] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                *reinterpret_cast<const float*>(vt + soff<U>(hr + 16 * i + 4 * g + j, 32 * ds + 2 * li)),
+                i ? y[j] : x[j], oacc[ds], 0, 0, 0);
+    } else if constexpr (RN == 32) {
+      const i16x8 pf = pack_frag(Mfma<T>::pack2(x[0], x[1]), Mfma<T>::pack2(x[2], x[3]), Mfma<T>::pack2(y[0], y[1]),
+                                 Mfma<T>::pack2(y[2], y[3]));
+#pragma unroll
+      for (int ds = 0; ds < DS; ++ds) oacc[ds] = Mfma<T>::mma(frag_tr<U>(vt, hr, 16 * ds, g, li), pf, oacc[ds]);
+    } else {
+      const u32x2 p = u32x2{Mfma<T>::pack2(x[0], x[1]), Mfma<T>::pack2(x[2], x[3])};
+#pragma unroll
+      for (int ds = 0; ds < DS; ++ds)
+        oacc[ds] = mma_k16<T>(lds_tr(vt + soff<U>(hr + 4 * g + (li >> 2), 16 * ds + 4 * (li & 3))),
+                              __builtin_bit_cast(i16x4, p), oacc[ds]);
     }
   };
-  int gi = g0 + w;
-  if (gi < g1) load(gi);
-
-  i16x8 qf[QT][KK];
-#pragma unroll
-  for (int qs = 0; qs < QT; ++qs)
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      const int i = 16 * qs + li, p = 4 * kk + g;
-      qf[qs][kk] = i16x8{0, 0, 0, 0, 0, 0, 0, 0};
-      if (i < N && p < cols)
-        qf[qs][kk] = *reinterpret_cast<const i16x8*>((const char*)((const T*)a.q + b * a.sq[0] + h * a.sq[1] + i * a.sq[2]) +
-                                                     16 * p);
-    }
-  __syncthreads();  // masks and depths
-  uint64_t anc[QT];
-  int qpos[QT];
-#pragma unroll
-  for (int qs = 0; qs < QT; ++qs) {
-    const int i = 16 * qs + li;
-    anc[qs] = i < N ? sanc[i] : 0ull;
-    qpos[qs] = 0;
-    if (i < N && n > 0) qpos[qs] = POS ? pp[c + i] : c + sdep[i];
-  }
-
-  f32x4 oacc[DS][QT];
-  float lsum[QT];
-#pragma unroll
-  for (int qs = 0; qs < QT; ++qs) {
-    lsum[qs] = 0.f;
-#pragma unroll
-    for (int ds = 0; ds < DS; ++ds) oacc[ds][qs] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  short* const vt = sv[w];
-
-  // one group from the loaded rows; TAIL: it reaches the tokens' rows or ends
-  // past the last filled row
-  auto work = [&](auto tail_tag, int k0, const i16x8 (&kc)[HH][KK]) __attribute__((always_inline)) {
-    constexpr bool TAIL = decltype(tail_tag)::value;
-    f32x4 f[HH][QT];
-#pragma unroll
-    for (int hh = 0; hh < HH; ++hh)
-#pragma unroll
-      for (int qs = 0; qs < QT; ++qs) {
-        f[hh][qs] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) f[hh][qs] = dot64<T>(kc[hh][kk], qf[qs][kk], f[hh][qs]);
-      }
-#pragma unroll
-    for (int hh = 0; hh < HH; ++hh)
+  // the same for 16 rows without 0 x inf: rows with f = 0 add nothing
+  auto product_checked = [&](int hr, const f32x4& x, const short* vt) __attribute__((always_inline)) {
+    for (int r = 0; r < 16; ++r) {
+      const int src = (r >> 2) * 16 + li;  // the lane that holds this row's f of query li
+      float y = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int row = k0 + 16 * hh + 4 * g + j;
-        const int tok = row - c;  // the drafted token in this row, if >= 0
-        int kpos = row;
-        if constexpr (POS) kpos = pp[TAIL ? min(row, n - 1) : row];
-        else if constexpr (TAIL) kpos = tok < 0 ? row : c + sdep[min(tok, kTreeMax - 1)];
-#pragma unroll
-        for (int qs = 0; qs < QT; ++qs) {
-          const float s = fmaf(f[hh][qs][j], scale, -slope * (float)(qpos[qs] - kpos));
-          float x = sig2_pow4(s);
-          if constexpr (TAIL) {
-            const bool seen = tok < 0 ? anc[qs] != 0ull : tok < N && ((anc[qs] >> (tok & 63)) & 1ull);
-            x = seen ? x : 0.f;
-          }
-          f[hh][qs][j] = x;
-          lsum[qs] += x;
-        }
+        const float z = __shfl(x[j], src, 64);
+        if ((r & 3) == j) y = z;
       }
-    bool plain = true;
-    if constexpr (TAIL) {
-      // values that some query must not see may be anything, and 0 x inf is not
-      // 0: a group holding a value that is not finite takes the products one by one
-      bool odd = false;
 #pragma unroll
-      for (int u = 0; u < NV; ++u) {
-        const VecT<T, 16 / ES> x = __builtin_bit_cast(VecT<T, 16 / ES>, vr[u]);
+      for (int ds = 0; ds < DS; ++ds)
 #pragma unroll
-        for (int e = 0; e < 16 / ES; ++e) odd = odd || !(fabsf((float)x.v[e]) <= 3.4028234e38f);
-      }
-      plain = __builtin_amdgcn_ballot_w64(odd) == 0ull;
-    }
-    if (plain) {
-      if constexpr (ES == 2) {
-        i16x8 pf[QT];
-#pragma unroll
-        for (int qs = 0; qs < QT; ++qs) {
-          const f32x4 x = f[0][qs], y = f[1][qs];
-          pf[qs] = pack_frag(Mfma<T>::pack2(x[0], x[1]), Mfma<T>::pack2(x[2], x[3]), Mfma<T>::pack2(y[0], y[1]),
-                             Mfma<T>::pack2(y[2], y[3]));
+        for (int j = 0; j < 4; ++j) {
+          const T z = *reinterpret_cast<const T*>(vt + soff<U>(hr + r, (16 * ds + 4 * g + j) * ES / 2));
+          if (y != 0.f) oacc[ds][j] = fmaf(y, (float)z, oacc[ds][j]);
         }
-#pragma unroll
-        for (int ds = 0; ds < DS; ++ds) {
-          const i16x8 vf = frag_tr<U>(vt, 0, 16 * ds, g, li);
-#pragma unroll
-          for (int qs = 0; qs < QT; ++qs) oacc[ds][qs] = Mfma<T>::mma(vf, pf[qs], oacc[ds][qs]);
-        }
-      } else {
-#pragma unroll
-        for (int ds = 0; ds < DS; ++ds)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float x = *reinterpret_cast<const float*>(vt + soff<U>(4 * g + j, 32 * ds + 2 * li));
-#pragma unroll
-            for (int qs = 0; qs < QT; ++qs)
-              oacc[ds][qs] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, f[0][qs][j], oacc[ds][qs], 0, 0, 0);
-          }
-      }
-    } else {
-      for (int r = 0; r < G; ++r) {
-        const int src = ((r & 15) >> 2) * 16 + li;  // the lane that holds this row's f of query li
-#pragma unroll
-        for (int qs = 0; qs < QT; ++qs) {
-          float x = 0.f;
-#pragma unroll
-          for (int hh = 0; hh < HH; ++hh)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float y = __shfl(f[hh][qs][j], src, 64);
-              if (r == 16 * hh + (r & 12) + j) x = y;
-            }
-#pragma unroll
-          for (int ds = 0; ds < DS; ++ds)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int d = 16 * ds + 4 * g + j;
-              const T y = *reinterpret_cast<const T*>(reinterpret_cast<const char*>(vt + soff<U>(r, d * ES / 2)));
-              if (x != 0.f) oacc[ds][qs][j] = fmaf(x, (float)y, oacc[ds][qs][j]);
-            }
-        }
-      }
     }
   };
 
-  for (; gi < g1; gi += kTreeWaves) {
-    const int k0 = gi * G;
-    i16x8 kc[HH][KK];
+  for (int t = t0; t < t1; ++t) {
+    // tile t has arrived once only the NS - 2 younger ones are in flight
+    if (t + NS - 2 < t1) dma_wait_but<(NS - 2) * OPS>();
+    else dma_wait();
+    __syncthreads();  // and every wave has left tile t - 1, whose stage is next
+    if (t + NS - 1 < t1) issue(t + NS - 1);
+    const int st = (t - t0) % NS, k0 = t * TR, h0 = kg * TK;
+    const short* const kt = ring + st * 2 * TR * U;
+    const short* const vt = kt + TR * U;
+    const int* const pt = &spos[POS ? st : 0][w][0];
+    if (k0 + TR <= c) {
 #pragma unroll
-    for (int hh = 0; hh < HH; ++hh)
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) kc[hh][kk] = kr[hh][kk];
-#pragma unroll
-    for (int u = 0; u < NV; ++u)
-      *reinterpret_cast<i16x8*>(vt + soff<U>(u * RPL + lane / CPR, 8 * (lane % CPR))) = vr[u];
-    if (k0 + G > c) {
-      work(std::true_type{}, k0, kc);
-      if (gi + kTreeWaves < g1) load(gi + kTreeWaves);
+      for (int hr = 0; hr < TK; hr += 32) {
+        const f32x4 x = scores(std::false_type{}, k0, h0 + hr, kt, pt);
+        if constexpr (TK >= 32) {
+          const f32x4 y = scores(std::false_type{}, k0, h0 + hr + 16, kt, pt);
+          product(std::integral_constant<int, 32>{}, h0 + hr, x, y, vt);
+        } else {
+          product(std::integral_constant<int, 16>{}, h0 + hr, x, x, vt);
+        }
+      }
     } else {
-      if (gi + kTreeWaves < g1) load(gi + kTreeWaves);
-      work(std::false_type{}, k0, kc);
+      for (int hr = h0; hr < h0 + TK; hr += 16) {
+        const f32x4 x = scores(std::true_type{}, k0, hr, kt, pt);
+        // values that some query must not see may be anything, and 0 x inf is
+        // not 0: rows that hold a value that is not finite go one by one
+        bool odd = false;
+#pragma unroll
+        for (int u = 0; u < U / 32; ++u) {
+          const VecT<T, 16 / ES> z = __builtin_bit_cast(VecT<T, 16 / ES>, lds16(vt + (hr + li) * U + 8 * (4 * u + g)));
+#pragma unroll
+          for (int e = 0; e < 16 / ES; ++e) odd = odd || !(fabsf((float)z.v[e]) <= 3.4028234e38f);
+        }
+        if (__builtin_amdgcn_ballot_w64(odd) == 0ull) product(std::integral_constant<int, 16>{}, hr, x, x, vt);
+        else product_checked(hr, x, vt);
+      }
     }
   }
 
-  // sums over the lane groups (l), then over the waves, in wave order
-#pragma unroll
-  for (int qs = 0; qs < QT; ++qs) {
-    lsum[qs] += __shfl_xor(lsum[qs], 16, 64);
-    lsum[qs] += __shfl_xor(lsum[qs], 32, 64);
-    if (g == 0) sl[w][16 * qs + li] = lsum[qs];
-  }
+  // L: over the lane groups; then, with the sums, over the row groups in order
+  lsum += __shfl_xor(lsum, 16, 64);
+  lsum += __shfl_xor(lsum, 32, 64);
+  const bool absent = anc == 0ull;
   const bool whole = a.splits == 1;
-  const int64_t prow = ((int64_t)bh * a.splits + split) * N;
+  const int64_t prow = ((int64_t)bh * a.splits + split) * N + qi;
+  T* const op = (T*)a.o + b * a.so[0] + h * a.so[1] + qi * a.so[2];
+  float l = lsum;
+  f32x4* const sx = reinterpret_cast<f32x4*>(ring);
+  if constexpr (KG > 1) {
+    if (g == 0) sl[w][li] = lsum;
+    __syncthreads();  // the ring is idle
 #pragma unroll
-  for (int qs = 0; qs < QT; ++qs) {
+    for (int ds = 0; ds < DS; ++ds) sx[(w * DS + ds) * 64 + lane] = oacc[ds];
     __syncthreads();
+    l = 0.f;
 #pragma unroll
-    for (int ds = 0; ds < DS; ++ds) sx[(w * DS + ds) * 64 + lane] = oacc[ds][qs];
-    __syncthreads();
-    const int i = 16 * qs + li;
-    float l = 0.f;
+    for (int i = 0; i < KG; ++i) l += sl[i * QG + qg][li];
+  }
+  if (absent) l = 0.f;
+  const float inv = 1.f / (l + 16.f * a.eps);
+  if (qi >= N) return;
+  if (kg == 0 && g == 0) {
+    if (!whole) a.lpart[prow] = l;
+    else if (a.L) a.L[(int64_t)bh * N + qi] = l * 0.0625f;
+  }
 #pragma unroll
-    for (int ww = 0; ww < kTreeWaves; ++ww) l += sl[ww][i];
-    const bool absent = anc[qs] == 0ull;
-    if (absent) l = 0.f;
-    const float inv = 1.f / (l + 16.f * a.eps);
-    if (i < N && w == 0 && g == 0) {
-      if (!whole) a.lpart[prow + i] = l;
-      else if (a.L) a.L[(int64_t)bh * N + i] = l * 0.0625f;
+  for (int ds = 0; ds < DS; ++ds) {
+    if (KG > 1 && ds % KG != kg) continue;  // a row group writes every KG-th subtile
+    f32x4 t = oacc[ds];
+    if constexpr (KG > 1) {
+      t = sx[(qg * DS + ds) * 64 + lane];
+#pragma unroll
+      for (int i = 1; i < KG; ++i) t += sx[((i * QG + qg) * DS + ds) * 64 + lane];
     }
-    for (int ds = w; ds < DS; ds += kTreeWaves) {
-      f32x4 t = sx[ds * 64 + lane];
-#pragma unroll
-      for (int ww = 1; ww < kTreeWaves; ++ww) t += sx[(ww * DS + ds) * 64 + lane];
-      if (absent) t = f32x4{0.f, 0.f, 0.f, 0.f};  // (their products with rows they do not see may be NaN)
-      const int d = 16 * ds + 4 * g;
-      if (i >= N) continue;
-      if (!whole) {
-        *reinterpret_cast<f32x4*>(a.part + (prow + i) * W + d) = t;
-      } else if (d < a.D) {
-        T* o = (T*)a.o + b * a.so[0] + h * a.so[1] + i * a.so[2] + d;
-        const float y[4] = {t[0] * inv, t[1] * inv, t[2] * inv, t[3] * inv};
-        store_acc<T, 4>(o, y);
-      }
+    if (absent) t = f32x4{0.f, 0.f, 0.f, 0.f};  // (its products with rows it does not see may be NaN)
+    const int d = 16 * ds + 4 * g;
+    if (!whole) {
+      *reinterpret_cast<f32x4*>(a.part + prow * W + d) = t;
+    } else if (d < a.D) {
+      const float y[4] = {t[0] * inv, t[1] * inv, t[2] * inv, t[3] * inv};
+      store_acc<T, 4>(op + d, y);
     }
   }
 }
@@ -392,16 +380,14 @@ template <typename T, int W> __global__ __launch_bounds__(kTreeCombThreads) void
 // Host side
 // ---------------------------------------------------------------------------
 
-// blocks per (b, h): enough to fill the CUs twice, none without a row group
-// per wave
-static int tree_splits(int64_t B, int64_t H, int64_t T, int dtype) {
-  const int per_block = kTreeWaves * (dtype == KAT_F32 ? 16 : 32);
+// blocks per (b, h): enough to fill the CUs twice, none without a tile
+static int tree_splits(int64_t B, int64_t H, int64_t T) {
   const int64_t want = (2 * (int64_t)num_cus() + B * H - 1) / (B * H);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(want, (T + per_block - 1) / per_block));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(want, (T + kTreeRows - 1) / kTreeRows));
 }
 
-template <typename T, int W, int QT, bool POS> static int launch_tree(const TreeArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((attn_tree_k<T, W, QT, POS>), dim3((unsigned)a.splits, (unsigned)(a.B * a.H)),
+template <typename T, int W, int QG, bool POS> static int launch_tree(const TreeArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((attn_tree_k<T, W, QG, POS>), dim3((unsigned)a.splits, (unsigned)(a.B * a.H)),
                      dim3(64 * kTreeWaves), 0, st, a);
   if (int rc = check_launch("kat_attn_tree")) return rc;
   if (a.splits == 1) return KAT_OK;
@@ -410,7 +396,7 @@ template <typename T, int W, int QT, bool POS> static int launch_tree(const Tree
                      st, a);
   return check_launch("kat_attn_tree (combine)");
 }
-template <typename T, int W> static int tree_qt(const TreeArgs& a, hipStream_t st) {
+template <typename T, int W> static int tree_qg(const TreeArgs& a, hipStream_t st) {
   const bool pos = a.positions != nullptr;
   if (a.N <= 16) return pos ? launch_tree<T, W, 1, true>(a, st) : launch_tree<T, W, 1, false>(a, st);
   if (a.N <= 32) return pos ? launch_tree<T, W, 2, true>(a, st) : launch_tree<T, W, 2, false>(a, st);
@@ -418,10 +404,10 @@ template <typename T, int W> static int tree_qt(const TreeArgs& a, hipStream_t s
 }
 template <typename T> static int tree_w(const TreeArgs& a, int W, hipStream_t st) {
   switch (W) {
-    case 32: if constexpr (sizeof(T) == 4) return tree_qt<T, 32>(a, st); break;
-    case 64: return tree_qt<T, 64>(a, st);
-    case 128: return tree_qt<T, 128>(a, st);
-    case 256: if constexpr (sizeof(T) == 2) return tree_qt<T, 256>(a, st); break;
+    case 32: if constexpr (sizeof(T) == 4) return tree_qg<T, 32>(a, st); break;
+    case 64: return tree_qg<T, 64>(a, st);
+    case 128: return tree_qg<T, 128>(a, st);
+    case 256: if constexpr (sizeof(T) == 2) return tree_qg<T, 256>(a, st); break;
   }
   return fail(KAT_EUNSUPPORTED, "kat_attn_tree: head dim %d", a.D);
 }
@@ -433,7 +419,7 @@ using namespace kat;
 extern "C" size_t kat_attn_tree_workspace_size(int64_t B, int64_t H, int64_t N, int64_t T, int64_t D, int dtype) {
   const int W = cache_layout(D, dtype);
   if (B <= 0 || H <= 0 || T <= 0 || N <= 0 || N > kTreeMax || !W) return 0;
-  const int splits = tree_splits(B, H, T, dtype);
+  const int splits = tree_splits(B, H, T);
   return splits == 1 ? 0 : (size_t)(B * H) * splits * N * (W + 1) * sizeof(float);
 }
 
@@ -458,6 +444,9 @@ extern "C" int kat_attn_tree(const void* q, const void* k, const void* v, void* 
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
     return fail(KAT_EUNSUPPORTED, "%s: tensors must be 16-byte aligned", nm);
   if (T > 1 && (strides[5] < D || strides[8] < D)) return fail(KAT_EINVAL, "%s: cache row stride < D", nm);
+  // a tile's rows are addressed by 31-bit byte offsets
+  if (T > 1 && std::max(strides[5], strides[8]) > 0x7fffffff / (kTreeRows * esz))
+    return fail(KAT_EUNSUPPORTED, "%s: cache row stride too large", nm);
   TreeArgs a = {};
   a.q = q;
   a.k = k;
@@ -479,6 +468,7 @@ extern "C" int kat_attn_tree(const void* q, const void* k, const void* v, void* 
     a.sv[i] = strides[6 + i];
     a.so[i] = strides[9 + i];
   }
+  if (T == 1) a.sk[2] = a.sv[2] = D;  // one row: its stride may be anything
   a.spar = parents_stride_b;
   if (positions) {
     a.spos[0] = pos_strides[0];
@@ -486,7 +476,7 @@ extern "C" int kat_attn_tree(const void* q, const void* k, const void* v, void* 
   }
   a.scale = scale;
   a.eps = eps;
-  a.splits = tree_splits(B, H, std::max<int64_t>(T, 1), dtype);
+  a.splits = tree_splits(B, H, std::max<int64_t>(T, 1));
   const size_t need = kat_attn_tree_workspace_size(B, H, N, T, D, dtype);
   if (need && (!workspace || workspace_bytes < need))
     return fail(KAT_EINVAL, "%s: workspace %zu bytes < required %zu", nm, workspace_bytes, need);
