@@ -756,15 +756,34 @@ std::optional<Tensor> key_weights(const Tensor& q, const Tensor& k, const Tensor
   return w;
 }
 
-// caches of one layout; the outputs are the inputs (in place) or other tensors.
-// The wrapper has checked shapes and types.
-void evict(const Tensor& k, const Tensor& v, const Tensor& w, const Tensor& p, const std::optional<Tensor>& n,
-           const Tensor& ko, const Tensor& vo, const Tensor& wo, const Tensor& po, const Tensor& no, int64_t keep,
-           int64_t recent, bool in_place) {
-  const c10::DeviceGuard dg(k.device());
+// The five tensors of a cache (k, v, weights, positions, lengths) into those of
+// another, or in place (out: none). False: something is not as the kernels take it
+bool evict(const Tensor& k, const Tensor& v, const Tensor& w, const Tensor& p, const std::optional<Tensor>& n,
+           const std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>>& out, int64_t keep, int64_t recent) {
+  if (!untraced() || !plain(k) || !same_place(k, {&v, &w}) || k.dim() != 4 || k.sizes() != v.sizes() ||
+      k.scalar_type() != v.scalar_type() || k.numel() == 0 || k.stride(3) != 1 || v.stride(3) != 1 ||
+      w.scalar_type() != at::kFloat || !ints(k, p) || (!n && !out) || keep < 0 || recent < 0 || recent > keep)
+    return false;
   const int64_t B = k.size(0), H = k.size(1), T = k.size(2), D = k.size(3);
-  const size_t wsb = kat_kv_evict_workspace_size(B, H, keep);
-  const Tensor ws = bytes(wsb, k);
+  if (!rows_ok(w, B, H, T) || !rows_ok(p, B, H, T) || !lengths_ok(k, n, B)) return false;
+  keep = std::min(keep, T);  // no sequence is longer
+  recent = std::min(recent, keep);
+  const Tensor &ko = out ? std::get<0>(*out) : k, &vo = out ? std::get<1>(*out) : v, &wo = out ? std::get<2>(*out) : w,
+               &po = out ? std::get<3>(*out) : p, &no = out ? std::get<4>(*out) : *n;
+  if (out) {
+    if (!same_place(k, {&ko, &vo, &wo}) || ko.dim() != 4) return false;
+    const int64_t S = ko.size(2);
+    if (S < keep || ko.sizes() != at::IntArrayRef({B, H, S, D}) || vo.sizes() != ko.sizes() ||
+        ko.scalar_type() != k.scalar_type() || vo.scalar_type() != k.scalar_type() || ko.stride(3) != 1 ||
+        vo.stride(3) != 1 || wo.scalar_type() != at::kFloat || !rows_ok(wo, B, H, S) || !ints(k, po) ||
+        !rows_ok(po, B, H, S) || !ints(k, no) || !no.is_contiguous() || no.dim() != 1 || no.numel() != B)
+      return false;
+  }
+  if (!apart(ko) || !apart(vo) || !apart(wo) || !apart(po)) return false;
+  at::NoGradGuard g;
+  const c10::DeviceGuard dg(k.device());
+  const size_t wsb = out ? 0 : kat_kv_evict_workspace_size(B, H, keep);
+  const Tensor ws = wsb ? bytes(wsb, k) : Tensor();
   int64_t s[20];
   int i = 0;
   for (const Tensor* t : {&k, &v, &ko, &vo})
@@ -773,9 +792,10 @@ void evict(const Tensor& k, const Tensor& v, const Tensor& w, const Tensor& p, c
     for (int d = 0; d < 2; ++d) s[i++] = t->stride(d);
   check(kat_kv_evict(k.data_ptr(), v.data_ptr(), w.data_ptr<float>(), p.data_ptr<int32_t>(),
                      n ? n->data_ptr<int32_t>() : nullptr, ko.data_ptr(), vo.data_ptr(), wo.data_ptr<float>(),
-                     po.data_ptr<int32_t>(), no.data_ptr<int32_t>(), ws.data_ptr(), wsb, B, H, T, D, keep, recent,
-                     in_place, s, code(k), stream(k)),
+                     po.data_ptr<int32_t>(), no.data_ptr<int32_t>(), wsb ? ws.data_ptr() : nullptr, wsb, B, H, T, D, keep,
+                     recent, !out, s, code(k), stream(k)),
         "kat_kv_evict");
+  return true;
 }
 
 }  // namespace

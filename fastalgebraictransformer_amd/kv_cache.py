@@ -209,44 +209,38 @@ def kv_cache_evict(k_cache, v_cache, weights, positions, lengths, keep, recent=0
     not in the order of their positions afterwards), and ``lengths`` becomes
     min(n, keep). With ``out`` = (k, v, weights, positions, lengths) of another
     cache with at least ``keep`` rows, the kept rows go there in their order and
-    the inputs stay as they are; rows behind them are left alone.
+    the inputs stay as they are (out's ``lengths`` too is another tensor than the
+    one given); rows behind them are left alone.
     Returns the five tensors that hold the result."""
-    B, H, T, D = k_cache.shape
-    assert k_cache.is_cuda and tuple(v_cache.shape) == (B, H, T, D) and v_cache.dtype == k_cache.dtype
-    assert 0 <= recent <= keep, "recent must lie in [0, keep]"
-    keep = min(int(keep), T)  # no sequence is longer
-    recent = min(int(recent), keep)
-    dev, dt = k_cache.device, k_cache.dtype
-    _lib.dtype_code(k_cache)
-    if out is None:
-        assert lengths is not None, "an eviction in place updates lengths"
-        _check_rows("k_cache", k_cache, (B, H, T, D), dt, dev)
-        _check_rows("v_cache", v_cache, (B, H, T, D), dt, dev)
-        _check_rows("weights", weights, (B, H, T), torch.float32, dev)
-        _check_rows("positions", positions, (B, H, T), torch.int32, dev)
-        _check_rows("lengths", lengths, (B,), torch.int32, dev)
-        k, v, w, p, n = k_cache, v_cache, weights, positions, lengths
-        res = (k, v, w, p, n)
-    else:
-        res = tuple(out)
-        assert len(res) == 5, "out must be (k, v, weights, positions, lengths)"
-        S = res[0].shape[2]
-        assert S >= keep, "out must have room for the kept rows"
-        _check_rows("out[0]", res[0], (B, H, S, D), dt, dev)
-        _check_rows("out[1]", res[1], (B, H, S, D), dt, dev)
-        _check_rows("out[2]", res[2], (B, H, S), torch.float32, dev)
-        _check_rows("out[3]", res[3], (B, H, S), torch.int32, dev)
-        _check_rows("out[4]", res[4], (B,), torch.int32, dev)
-        k, v = _unit_d(k_cache), _unit_d(v_cache.to(dev))
-        assert tuple(weights.shape) == (B, H, T), f"weights must be [B, H, T] = [{B}, {H}, {T}]"
-        w = _unit_t(weights.to(device=dev, dtype=torch.float32))
-        p = _positions_arg(positions, B, H, T, k)
-        assert p is not None, "positions are required"
-        n = _lengths_arg(lengths, k)
-    if B * H == 0:
+    assert k_cache.is_cuda and v_cache.is_cuda
+    if out is not None:
+        out = tuple(out)
+        assert len(out) == 5, "out must be (k, v, weights, positions, lengths)"
+    res = (k_cache, v_cache, weights, positions, lengths) if out is None else out
+    if _lib.ops().evict(k_cache, v_cache, weights, positions, lengths, out, keep, recent):
         return res
-    if T == 0:  # nothing to move
+    B, H, T, D = k_cache.shape
+    assert tuple(v_cache.shape) == (B, H, T, D) and v_cache.dtype == k_cache.dtype
+    assert 0 <= recent <= keep, "recent must lie in [0, keep]"
+    assert out is not None or lengths is not None, "an eviction in place updates lengths"
+    dev, dt, S = k_cache.device, k_cache.dtype, res[0].shape[2]
+    _lib.dtype_code(k_cache)
+    # what is written cannot be converted
+    for name, t, shape, dtype in (("k", res[0], (B, H, S, D), dt), ("v", res[1], (B, H, S, D), dt),
+                                  ("weights", res[2], (B, H, S), torch.float32),
+                                  ("positions", res[3], (B, H, S), torch.int32),
+                                  ("lengths", res[4], (B,), torch.int32)):
+        _check_rows(name if out is None else f"out's {name}", t, shape, dtype, dev)
+    assert S >= min(keep, T), "out must have room for the kept rows"
+    if B * H * T * D == 0:  # nothing to move
         res[4].zero_()
         return res
-    _lib.ops().evict(k, v, w, p, n, *res, keep, recent, out is None)
+    if out is not None:
+        assert tuple(weights.shape) == (B, H, T), f"weights must be [B, H, T] = [{B}, {H}, {T}]"
+        k_cache, v_cache = _unit_d(k_cache), _unit_d(v_cache.to(dev))
+        weights = _unit_t(weights.to(device=dev, dtype=torch.float32))
+        positions = _positions_arg(positions, B, H, T, k_cache)
+        lengths = _lengths_arg(lengths, k_cache)
+    if not _lib.ops().evict(k_cache, v_cache, weights, positions, lengths, out, keep, recent):
+        raise RuntimeError("kv_cache_evict takes plain CUDA tensors only")
     return res

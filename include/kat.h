@@ -348,12 +348,12 @@ int kat_attn_key_weights(const void* q, const void* k, const float* L, float* we
  * NULL) becomes m.
  *   in_place == 0: the kept rows of k, v, weights, positions go to rows 0 .. m - 1
  *     of the outputs (at least min(T, keep) rows each), in their order; the
- *     outputs must not overlap the inputs, and rows at or past m are left alone.
+ *     outputs, lengths_out among them, must not overlap the inputs, and rows at or past m are left alone.
  *   in_place != 0: the outputs are the inputs; kept rows below m stay, the kept
  *     rows at or past m move, in order, into the given-up rows below m.
  * k, v: [B, H, T, D] of dtype, any head dim of whole 16-byte pieces, 16-byte
- * aligned rows; weights fp32 and positions int32 [B, H, T], unit t-stride.
- * strides: 20 int64 = (b, h, t) of k, v, k_out, v_out, then (b, h) of weights,
+ * aligned rows; weights fp32 and positions int32 [B, H, T], unit t-stride. T = 0 is
+ * a no-op. Only the call in place needs the workspace. strides: 20 int64 = (b, h, t) of k, v, k_out, v_out, then (b, h) of weights,
  * positions, weights_out, positions_out. recent <= keep. */
 size_t kat_kv_evict_workspace_size(int64_t B, int64_t H, int64_t keep);
 int kat_kv_evict(const void* k, const void* v, const float* weights, const int32_t* positions,

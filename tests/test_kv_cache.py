@@ -92,5 +92,8 @@ def test_evict_refusals():
     assert call(dtype=9) == 2 and call(keep=-1) == 1
     assert call(in_place=1) == 1 and "in place" in _msg()
     assert call(out=None) == 1 and "null" in _msg()
-    assert call() == 1 and "workspace" in _msg()
+    assert call(T=0) == 0
+    assert call(in_place=1, out=P) == 1 and "workspace" in _msg()
+    assert lib.kat_kv_evict(P, P, P, P, P, P, P, P, P, P, None, 0, 1, 2, 9, 64, 4, 0, 0, _lib.i64_array([64] * 20), 1,
+                            None) == 1 and "lengths_out" in _msg()
     assert lib.kat_kv_evict_workspace_size(2, 3, 10) == 6 * 21 * 4
