@@ -19,6 +19,7 @@
 // second kernel adds the splits in a fixed order. No atomics.
 
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "attn_cache.h"
@@ -46,17 +47,21 @@ struct KeywArgs {
 constexpr int kKwWaves = 4;
 // a row in 16-bit units
 template <typename T, int W> constexpr int kw_units() { return W * (int)sizeof(T) / 2; }
-// 16-key subtiles per wave: their fragments take U / 8 registers each
-template <int U> constexpr int kw_ks() { return U <= 128 ? 4 : U == 256 ? 2 : 1; }
 // query rows per LDS tile
 template <int U> constexpr int kw_rows() { return U == 512 ? 32 : 64; }
 
-template <typename T, int W, bool KM>
+// KS: 16-key subtiles per wave (their fragments take U / 8 registers each). QW:
+// waves that share their keys and split a tile's queries (1 or 4)
+template <typename T, int W, bool KM, int KS, int QW>
 __global__ __launch_bounds__(64 * kKwWaves, (kw_units<T, W>() == 512 ? 1 : 2)) void attn_keyw_k(KeywArgs a) {
-  constexpr int ES = (int)sizeof(T), U = kw_units<T, W>(), KK = U / 32, KS = kw_ks<U>(), QR = kw_rows<U>();
-  constexpr int BK = 16 * KS * kKwWaves;  // keys per block
+  constexpr int ES = (int)sizeof(T), U = kw_units<T, W>(), KK = U / 32, QR = kw_rows<U>() * (QW == 4 && U == 512 ? 2 : 1);
+  constexpr int KWV = kKwWaves / QW;   // waves with keys of their own
+  constexpr int BK = 16 * KS * KWV;    // keys per block
+  constexpr int WR = QR / QW;          // rows of a tile per wave
+  constexpr bool kBiasC = ES == 2;     // the bias enters the product as its C operand
   __shared__ short sq[2][QR * U];
   __shared__ float sc[2][QR];  // 1 / (16 (L + eps)) of the tile's queries; 0: the query does not count
+  __shared__ float sw[QW][BK];
 
   int bh, kb;
   block_order((int)blockIdx.x, a.B * a.H, bh, kb);
@@ -67,14 +72,17 @@ __global__ __launch_bounds__(64 * kKwWaves, (kw_units<T, W>() == 512 ? 1 : 2)) v
   if (r0 >= r1) return;  // fewer chunks than the longest key block has
   const int lane = threadIdx.x & 63, w = wave_id();
   const int g = lane >> 4, li = lane & 15;
-  const int kw = kb * BK + w * 16 * KS;  // the wave's first key
+  const int kw = kb * BK + (w % KWV) * 16 * KS;  // the wave's first key
+  const int w0 = (w / KWV) * WR;                 // its first row of a tile
 
   const char* qp = (const char*)((const T*)a.q + b * a.sq[0] + h * a.sq[1]);
   const char* kp = (const char*)((const T*)a.k + b * a.sk[0] + h * a.sk[1]);
   const int64_t sqb = a.sq[2] * ES, skb = a.sk[2] * ES;
   const float* lp = a.L + b * a.sl[0] + h * a.sl[1];
   const uint8_t* mp = KM ? a.mask + b * a.smask : nullptr;
-  const float slope = a.slopes[h], scale = a.scale;
+  const float slope = a.slopes[h];
+  // (a scale below 2^-60 moves no score, but the bias is divided by it)
+  const float scale = !kBiasC || fabsf(a.scale) >= 0x1p-60f ? a.scale : copysignf(0x1p-60f, a.scale);
   const int cols = a.D * ES / 16;
 
   TileDma<U, kKwWaves, QR> dq;
@@ -101,23 +109,26 @@ __global__ __launch_bounds__(64 * kKwWaves, (kw_units<T, W>() == 512 ? 1 : 2)) v
         kf[ks][kk] = *reinterpret_cast<const i16x8*>(kp + (int64_t)std::min(kw + 16 * ks + li, T_ - 1) * skb + 16 * p);
     }
   if (threadIdx.x < QR) sc[0][threadIdx.x] = cinv(r0 + (int)threadIdx.x);
-  float bl[4];  // slope (key - q) of a 16 x 16 piece: the lane's part
+  // slope (key - q) of a 16 x 16 piece: the lane's part, for the product divided
+  // by the scale (fp32: added after it, or it would set the rounding of the sums)
+  f32x4 bl;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) bl[j] = slope * (float)(li - 4 * g - j);
+  for (int j = 0; j < 4; ++j) bl[j] = (kBiasC ? slope / scale : slope) * (float)(li - 4 * g - j);
   f32x4 acc[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) acc[ks] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // the tile's rows row .. row + QR - 1 against the wave's keys. MASKED: it
-  // touches the diagonal or holds a query that does not count (whose values may
-  // be anything)
+  // the wave's rows of a tile, row .. row + WR - 1, against its keys. MASKED: they
+  // touch the diagonal or hold a query that does not count (whose values may be
+  // anything)
   auto tile = [&](auto masked_tag, int row, const short* qt, const float* ct) __attribute__((always_inline)) {
     constexpr bool MASKED = decltype(masked_tag)::value;
+    const float base = slope * (float)(kw - row);
 #pragma unroll
-    for (int hr = 0; hr < QR; hr += 16) {
+    for (int hr = 0; hr < WR; hr += 16) {
       f32x4 s_[KS];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s_[ks] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int ks = 0; ks < KS; ++ks) s_[ks] = kBiasC ? bl : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         const i16x8 qa = lds16(qt + soff<U>(hr + li, 32 * kk + 8 * g));
@@ -127,10 +138,10 @@ __global__ __launch_bounds__(64 * kKwWaves, (kw_units<T, W>() == 512 ? 1 : 2)) v
       const f32x4 c = *reinterpret_cast<const f32x4*>(ct + hr + 4 * g);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const float tterm = slope * (float)(kw + 16 * ks - row - hr);
+        const float tterm = fmaf(slope, (float)(16 * ks - hr), base);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float s = fmaf(s_[ks][j], scale, bl[j] + tterm);
+          const float s = fmaf(s_[ks][j], scale, kBiasC ? tterm : bl[j] + tterm);
           const float r = __builtin_amdgcn_rcpf(fabsf(s) + 1.f);
           const float t = fmaf(s, r, 1.f);
           const float t2 = t * t;
@@ -156,11 +167,12 @@ __global__ __launch_bounds__(64 * kKwWaves, (kw_units<T, W>() == 512 ? 1 : 2)) v
       issue(sq[buf ^ 1], row + QR);
       if (threadIdx.x < QR) cn = cinv(row + QR + (int)threadIdx.x);
     }
-    if (row + QR - 1 >= kw) {  // else every key of the wave lies past the tile's queries
-      bool plain = row >= kw + 16 * KS - 1;
-      if constexpr (KM) plain = plain && __builtin_amdgcn_ballot_w64(lane < QR && sc[buf][lane % QR] == 0.f) == 0ull;
-      if (plain) tile(std::false_type{}, row, sq[buf], sc[buf]);
-      else tile(std::true_type{}, row, sq[buf], sc[buf]);
+    const int rw = row + w0;
+    if (rw + WR - 1 >= kw) {  // else every key of the wave lies past its queries
+      bool plain = rw >= kw + 16 * KS - 1;
+      if constexpr (KM) plain = plain && __builtin_amdgcn_ballot_w64(lane < WR && sc[buf][w0 + lane % WR] == 0.f) == 0ull;
+      if (plain) tile(std::false_type{}, rw, sq[buf] + w0 * U, sc[buf] + w0);
+      else tile(std::true_type{}, rw, sq[buf] + w0 * U, sc[buf] + w0);
     }
     if (more && threadIdx.x < QR) sc[buf ^ 1][threadIdx.x] = cn;
     dma_wait();
@@ -176,12 +188,17 @@ __global__ __launch_bounds__(64 * kKwWaves, (kw_units<T, W>() == 512 ? 1 : 2)) v
     float t = (acc[ks][0] + acc[ks][1]) + (acc[ks][2] + acc[ks][3]);
     t += __shfl_xor(t, 16, 64);
     t += __shfl_xor(t, 32, 64);
-    const int key = kw + 16 * ks + li;
-    if (g == 0 && key < T_) {
-      if (KM && mp[key] == 0) t = 0.f;
-      if (a.part) a.part[((int64_t)blockIdx.y * a.B * a.H + bh) * T_ + key] = t;
-      else a.out[b * a.so[0] + h * a.so[1] + key] = t;
-    }
+    if (g == 0) sw[w / KWV][(w % KWV) * 16 * KS + 16 * ks + li] = t;
+  }
+  __syncthreads();
+  const int key = kb * BK + (int)threadIdx.x;
+  if ((int)threadIdx.x < BK && key < T_) {
+    float t = sw[0][threadIdx.x];
+#pragma unroll
+    for (int i = 1; i < QW; ++i) t += sw[i][threadIdx.x];
+    if (KM && mp[key] == 0) t = 0.f;
+    if (a.part) a.part[((int64_t)blockIdx.y * a.B * a.H + bh) * T_ + key] = t;
+    else a.out[b * a.so[0] + h * a.so[1] + key] = t;
   }
 }
 
@@ -216,38 +233,54 @@ static int keyw_layout(int64_t D, int dtype) {
   if (dtype == KAT_F32 && D > 128 && D <= 256 && D % 4 == 0) return 256;
   return cache_layout(D, dtype);
 }
-static int keyw_block_keys(int W, int dtype) {
+// How a call is laid out: keys per block (ks 16-key subtiles per wave, qw waves
+// per key set), queries per block and their number of chunks.
+struct KeywPlan {
+  int ks, qw, bk, qc, chunks;
+};
+static KeywPlan keyw_plan(int64_t B, int64_t H, int64_t T, int64_t lo, int W, int dtype) {
   const int U = W * dtype_size(dtype) / 2;
-  return 16 * kKwWaves * (U <= 128 ? 4 : U == 256 ? 2 : 1);
-}
-
-// queries per block: about four blocks per CU, whole 64-row tiles
-static void keyw_plan(int64_t B, int64_t H, int64_t T, int64_t lo, int W, int dtype, int& qc, int& chunks) {
-  const int64_t bk = keyw_block_keys(W, dtype);
+  KeywPlan p = {U <= 128 ? 4 : U == 256 ? 2 : 1, 1, 0, 0, 0};
+  const char* e = getenv("KW_MODE");
+  if (e && e[0] == '1') p.ks = 1;
+  if (e && e[0] == '2') { p.ks = 1; p.qw = 4; }
+  if (e && e[0] == '3') { p.ks = 2; p.qw = 4; }
+  if (e && e[0] == '4') { p.ks = 2; p.qw = 1; }
+  p.bk = 16 * p.ks * kKwWaves / p.qw;
   int64_t rows = 0;  // (key block, query row) pairs of one head
-  for (int64_t k = 0; k < T; k += bk) rows += T - std::max(lo, k);
-  int64_t c = (rows * B * H + 4 * num_cus() - 1) / (4 * num_cus());
+  for (int64_t k = 0; k < T; k += p.bk) rows += T - std::max(lo, k);
+  const int per = getenv("KW_PER") ? atoi(getenv("KW_PER")) : 4;
+  int64_t c = (rows * B * H + per * num_cus() - 1) / (per * num_cus());
   c = std::max<int64_t>(64, (c + 63) / 64 * 64);
-  chunks = (int)((T - lo + c - 1) / c);
-  qc = (int)std::min<int64_t>(c, 0x3fffffc0);
+  if (getenv("KW_QC")) c = atoi(getenv("KW_QC"));
+  p.chunks = (int)((T - lo + c - 1) / c);
+  p.qc = (int)std::min<int64_t>(c, 0x3fffffc0);
+  return p;
 }
 
-template <typename T, int W> static int launch_keyw(const KeywArgs& a, hipStream_t st) {
-  constexpr int U = kw_units<T, W>(), BK = 16 * kw_ks<U>() * kKwWaves;
+template <typename T, int W, int KS, int QW> static int launch_keyw(const KeywArgs& a, hipStream_t st) {
+  constexpr int BK = 16 * KS * kKwWaves / QW;
   const dim3 grid((unsigned)((a.T + BK - 1) / BK * a.B * a.H), (unsigned)a.chunks);
-  if (a.mask) hipLaunchKernelGGL((attn_keyw_k<T, W, true>), grid, dim3(64 * kKwWaves), 0, st, a);
-  else hipLaunchKernelGGL((attn_keyw_k<T, W, false>), grid, dim3(64 * kKwWaves), 0, st, a);
+  if (a.mask) hipLaunchKernelGGL((attn_keyw_k<T, W, true, KS, QW>), grid, dim3(64 * kKwWaves), 0, st, a);
+  else hipLaunchKernelGGL((attn_keyw_k<T, W, false, KS, QW>), grid, dim3(64 * kKwWaves), 0, st, a);
   if (int rc = check_launch("kat_attn_key_weights")) return rc;
   if (!a.part) return KAT_OK;
   hipLaunchKernelGGL(attn_keyw_sum_k, dim3((unsigned)((a.T + 255) / 256), (unsigned)(a.B * a.H)), dim3(256), 0, st, a, BK);
   return check_launch("kat_attn_key_weights (sum)");
 }
-template <typename T> static int keyw_w(const KeywArgs& a, int W, hipStream_t st) {
+template <typename T, int W> static int keyw_mode(const KeywArgs& a, const KeywPlan& p, hipStream_t st) {
+  if (p.qw == 4) return p.ks == 2 ? launch_keyw<T, W, 2, 4>(a, st) : launch_keyw<T, W, 1, 4>(a, st);
+  if (p.ks == 1) return launch_keyw<T, W, 1, 1>(a, st);
+  if constexpr (kw_units<T, W>() <= 256) { if (p.ks == 2) return launch_keyw<T, W, 2, 1>(a, st); }
+  if constexpr (kw_units<T, W>() <= 128) return launch_keyw<T, W, 4, 1>(a, st);
+  return KAT_EINVAL;
+}
+template <typename T> static int keyw_w(const KeywArgs& a, int W, const KeywPlan& p, hipStream_t st) {
   switch (W) {
-    case 32: if constexpr (sizeof(T) == 4) return launch_keyw<T, 32>(a, st); break;
-    case 64: return launch_keyw<T, 64>(a, st);
-    case 128: return launch_keyw<T, 128>(a, st);
-    case 256: return launch_keyw<T, 256>(a, st);
+    case 32: if constexpr (sizeof(T) == 4) return keyw_mode<T, 32>(a, p, st); break;
+    case 64: return keyw_mode<T, 64>(a, p, st);
+    case 128: return keyw_mode<T, 128>(a, p, st);
+    case 256: return keyw_mode<T, 256>(a, p, st);
   }
   return fail(KAT_EUNSUPPORTED, "kat_attn_key_weights: head dim %d", a.D);
 }
@@ -260,8 +293,7 @@ extern "C" size_t kat_attn_key_weights_workspace_size(int64_t B, int64_t H, int6
                                                       int dtype) {
   const int W = keyw_layout(D, dtype);
   if (B <= 0 || H <= 0 || T <= 0 || last < 0 || !W) return 0;
-  int qc, chunks;
-  keyw_plan(B, H, T, last == 0 ? 0 : std::max<int64_t>(0, T - last), W, dtype, qc, chunks);
+  const int chunks = keyw_plan(B, H, T, last == 0 ? 0 : std::max<int64_t>(0, T - last), W, dtype).chunks;
   return chunks == 1 ? 0 : (size_t)chunks * B * H * T * sizeof(float);
 }
 
@@ -308,17 +340,19 @@ extern "C" int kat_attn_key_weights(const void* q, const void* k, const float* L
   a.so[1] = strides[10];
   a.scale = scale;
   a.eps = eps;
-  keyw_plan(B, H, T, a.lo, W, dtype, a.qc, a.chunks);
+  const KeywPlan p = keyw_plan(B, H, T, a.lo, W, dtype);
+  a.qc = p.qc;
+  a.chunks = p.chunks;
   const size_t need = kat_attn_key_weights_workspace_size(B, H, T, D, last, dtype);
   if (need && (!workspace || workspace_bytes < need))
     return fail(KAT_EINVAL, "%s: workspace %zu bytes < required %zu", nm, workspace_bytes, need);
   a.part = need ? (float*)workspace : nullptr;
-  if (a.chunks > 0xffff || (T + 63) / 64 * B * H > 0x7fffffff) return fail(KAT_EUNSUPPORTED, "%s: B*H*T too large", nm);
+  if (a.chunks > 0xffff || (T + 15) / 16 * B * H > 0x7fffffff) return fail(KAT_EUNSUPPORTED, "%s: B*H*T too large", nm);
   const hipStream_t st = as_stream(stream);
   switch (dtype) {
-    case KAT_F32: return keyw_w<float>(a, W, st);
-    case KAT_BF16: return keyw_w<bf16>(a, W, st);
-    case KAT_F16: return keyw_w<f16>(a, W, st);
+    case KAT_F32: return keyw_w<float>(a, W, p, st);
+    case KAT_BF16: return keyw_w<bf16>(a, W, p, st);
+    case KAT_F16: return keyw_w<f16>(a, W, p, st);
   }
   return fail(KAT_EUNSUPPORTED, "%s: unsupported dtype %d", nm, dtype);
 }

@@ -84,10 +84,16 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int b, int h, int 
   const int t = threadIdx.x;
   auto to = [&](int i) __attribute__((always_inline)) { return dst ? dst[i] : first + i; };
   const int rows = last - first;
-  for (int i = t; i < rows; i += NT) {
-    const int s = src[i], d = to(i);
-    a.wo[b * a.swo[0] + h * a.swo[1] + d] = a.w[b * a.sw[0] + h * a.sw[1] + s];
-    a.po[b * a.spo[0] + h * a.spo[1] + d] = a.pos[b * a.spos[0] + h * a.spos[1] + s];
+  // the totals and positions: their loads run beside those of the first pieces
+  const float* w = a.w + b * a.sw[0] + h * a.sw[1];
+  const int32_t* pos = a.pos + b * a.spos[0] + h * a.spos[1];
+  float* wo = a.wo + b * a.swo[0] + h * a.swo[1];
+  int32_t* po = a.po + b * a.spo[0] + h * a.spo[1];
+  float w0 = 0.f;
+  int32_t p0 = 0;
+  if (t < rows) {
+    w0 = w[src[t]];
+    p0 = pos[src[t]];
   }
   const char* k = a.k + b * a.sk[0] + h * a.sk[1];
   const char* v = a.v + b * a.sv[0] + h * a.sv[1];
@@ -118,6 +124,14 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int b, int h, int 
         *reinterpret_cast<mfma::i16x8*>(ko + (int64_t)at[u] * a.sko[2] + 16 * pc[u]) = x[u];
         *reinterpret_cast<mfma::i16x8*>(vo + (int64_t)at[u] * a.svo[2] + 16 * pc[u]) = y[u];
       }
+  }
+  if (t < rows) {
+    wo[to(t)] = w0;
+    po[to(t)] = p0;
+  }
+  for (int i = t + NT; i < rows; i += NT) {
+    wo[to(i)] = w[src[i]];
+    po[to(i)] = pos[src[i]];
   }
 }
 
@@ -401,11 +415,14 @@ extern "C" int kat_kv_evict(const void* k, const void* v, const float* weights, 
   a.cnt = a.dst + (size_t)(B * H) * keep;
   const hipStream_t st = as_stream(stream);
   const bool one = !in_place;
-  // as many blocks as CUs, of at least 32 rows each
-  const int64_t want = (num_cus() + B * H - 1) / (B * H), rows = std::max<int64_t>(1, std::min(keep, T));
+  // a block per CU (each selects anew, so a second one on a CU costs more than it
+  // brings: 23 against 18.6 us at B=16, H=12, T=2048, keep 512), at least 32 rows each
+  const int64_t want = std::max<int64_t>(1, num_cus() / (B * H)), rows = std::max<int64_t>(1, std::min(keep, T));
   a.share = (int)std::min<int64_t>(kEvShare, std::max<int64_t>(32, (rows + want - 1) / want));
-  // few rows: few waves, whose barriers are cheaper; many: all the waves of a CU
-  if (T <= 1024) return launch_evict<256, 4>(a, one, st);
+  // waves enough that a thread holds few keys (640 rows: 256 threads of 4 keys 6.6 us,
+  // 512 of 2 5.9, 1024 of 1 6.3; 2048 rows: 1024 of 2 7.1, 512 of 8 7.8, 256 of 16 9.7)
+  if (T <= 1024) return launch_evict<512, 2>(a, one, st);
+  if (T <= 2048) return launch_evict<1024, 2>(a, one, st);
   if (T <= 4096) return launch_evict<1024, 4>(a, one, st);
   if (T <= 16384) return launch_evict<1024, 16>(a, one, st);
   if (T <= 32768) return launch_evict<1024, 32>(a, one, st);
