@@ -6,7 +6,7 @@
 // a dropped token neither gives nor receives weight. This is what an eviction
 // policy needs of a prompt before its keys go into a smaller cache.
 //
-// Design (MI355X). One matrix product and ~9 VALU operations per (query, key)
+// Design (MI355X). One matrix product and 8 VALU operations per (query, key)
 // pair and no output but T floats per head: instruction issue (MFMA + VALU)
 // bounds it, not memory. Like the backward's dK/dV pass a block keeps its keys'
 // fragments in registers and streams the queries through LDS (64-row tiles,
@@ -14,12 +14,11 @@
 //   S[q][key] = Q K^T   A = Q rows (ds_read_b128), B = K (registers)
 // and a lane holds queries 4 g + j of its key li, so the column sums stay in
 // registers until the end (lane groups added by two shuffles). Every Q fragment
-// read feeds the products of KS 16-key subtiles. Queries are split over
-// blocks (QC rows each) so that the causal triangle fills the chip evenly; a
-// second kernel adds the splits in a fixed order. No atomics.
+// read feeds the products of KS 16-key subtiles. Grids short of the chip split the
+// queries over the waves of a block or over blocks, whose sums are added in a
+// fixed order (keyw_plan has the rules and what they measured). No atomics.
 
 #include <algorithm>
-#include <cstdlib>
 #include <type_traits>
 
 #include "attn_cache.h"
@@ -234,27 +233,42 @@ static int keyw_layout(int64_t D, int dtype) {
   return cache_layout(D, dtype);
 }
 // How a call is laid out: keys per block (ks 16-key subtiles per wave, qw waves
-// per key set), queries per block and their number of chunks.
+// per key set), queries per block and their number of chunks. Measured (GPU time,
+// us, causal, every query unless said):
+//  - Own keys per wave, 16 or (16-bit types, large calls) 32 of them: more keys per Q
+//    read against more waves per SIMD. bf16 16 / 32 / 64 keys: 64 heads, T=4096, D=128
+//    214 / 194 / 219; 192 heads, T=2048, D=64 119 / 114 / 122, of which the last 64
+//    queries 15.8 / 13.9 / 14.6; 48 heads, T=2048 35 / 37 / 43; 64 heads, T=1000, D=96
+//    19.4 / 21.5 / 25. fp32, T=2048: 32 heads of 128 172 / 180, 12 of 64 44.8 / 44.9.
+//  - With fewer than three such blocks per CU the queries are split too. Up to 1024
+//    rows over the four waves of a block that share 16 keys, in one launch: bf16, D=64,
+//    chunks / waves: 12 heads, T=256 5.9 / 4.3; 48 heads, T=512 9.3 / 7.6; 24 heads,
+//    T=1000 12.3 / 10.9 (12 heads 9.6 / 9.9, and 16.6 / 18.4 at T=2048). Beyond, in
+//    chunks over blocks, about four per CU, and a second launch: fp32, 12 heads,
+//    T=2048 53 us in two chunks, 44.8 in six.
+//  - Else one block takes all its queries, the longest first (64 heads, T=4096: 194 us
+//    whole, 207 in two chunks; 96 heads, T=512 8.9 whole, 11.7 split over waves).
 struct KeywPlan {
   int ks, qw, bk, qc, chunks;
 };
-static KeywPlan keyw_plan(int64_t B, int64_t H, int64_t T, int64_t lo, int W, int dtype) {
-  const int U = W * dtype_size(dtype) / 2;
-  KeywPlan p = {U <= 128 ? 4 : U == 256 ? 2 : 1, 1, 0, 0, 0};
-  const char* e = getenv("KW_MODE");
-  if (e && e[0] == '1') p.ks = 1;
-  if (e && e[0] == '2') { p.ks = 1; p.qw = 4; }
-  if (e && e[0] == '3') { p.ks = 2; p.qw = 4; }
-  if (e && e[0] == '4') { p.ks = 2; p.qw = 1; }
-  p.bk = 16 * p.ks * kKwWaves / p.qw;
+static KeywPlan keyw_plan(int64_t B, int64_t H, int64_t T, int64_t lo, int dtype) {
+  const int64_t cus = num_cus(), bh = B * H;
+  KeywPlan p = {1, 1, 0, 0, 0};
+  const double pairs = (double)bh * ((double)(T - lo) * lo + 0.5 * (T - lo) * (T - lo));
+  if (dtype != KAT_F32 && (pairs >= 0x1p27 || (T + 127) / 128 * bh >= 8 * cus)) p.ks = 2;
+  p.bk = 16 * p.ks * kKwWaves;
   int64_t rows = 0;  // (key block, query row) pairs of one head
   for (int64_t k = 0; k < T; k += p.bk) rows += T - std::max(lo, k);
-  const int per = getenv("KW_PER") ? atoi(getenv("KW_PER")) : 4;
-  int64_t c = (rows * B * H + per * num_cus() - 1) / (per * num_cus());
-  c = std::max<int64_t>(64, (c + 63) / 64 * 64);
-  if (getenv("KW_QC")) c = atoi(getenv("KW_QC"));
+  int64_t c = T - lo;
+  if ((T + p.bk - 1) / p.bk * bh < 3 * cus) c = std::max<int64_t>(64, (rows * bh + 4 * cus - 1) / (4 * cus));
+  c = (c + 63) / 64 * 64;  // whole tiles
+  if (c < T - lo && p.ks == 1 && T <= 1024) {
+    p.qw = kKwWaves;
+    p.bk = 16;
+    c = (T - lo + 63) / 64 * 64;
+  }
   p.chunks = (int)((T - lo + c - 1) / c);
-  p.qc = (int)std::min<int64_t>(c, 0x3fffffc0);
+  p.qc = (int)c;
   return p;
 }
 
@@ -269,11 +283,11 @@ template <typename T, int W, int KS, int QW> static int launch_keyw(const KeywAr
   return check_launch("kat_attn_key_weights (sum)");
 }
 template <typename T, int W> static int keyw_mode(const KeywArgs& a, const KeywPlan& p, hipStream_t st) {
-  if (p.qw == 4) return p.ks == 2 ? launch_keyw<T, W, 2, 4>(a, st) : launch_keyw<T, W, 1, 4>(a, st);
-  if (p.ks == 1) return launch_keyw<T, W, 1, 1>(a, st);
-  if constexpr (kw_units<T, W>() <= 256) { if (p.ks == 2) return launch_keyw<T, W, 2, 1>(a, st); }
-  if constexpr (kw_units<T, W>() <= 128) return launch_keyw<T, W, 4, 1>(a, st);
-  return KAT_EINVAL;
+  if (p.qw == kKwWaves) return launch_keyw<T, W, 1, kKwWaves>(a, st);
+  if constexpr (sizeof(T) == 2) {
+    if (p.ks == 2) return launch_keyw<T, W, 2, 1>(a, st);
+  }
+  return launch_keyw<T, W, 1, 1>(a, st);
 }
 template <typename T> static int keyw_w(const KeywArgs& a, int W, const KeywPlan& p, hipStream_t st) {
   switch (W) {
@@ -293,7 +307,7 @@ extern "C" size_t kat_attn_key_weights_workspace_size(int64_t B, int64_t H, int6
                                                       int dtype) {
   const int W = keyw_layout(D, dtype);
   if (B <= 0 || H <= 0 || T <= 0 || last < 0 || !W) return 0;
-  const int chunks = keyw_plan(B, H, T, last == 0 ? 0 : std::max<int64_t>(0, T - last), W, dtype).chunks;
+  const int chunks = keyw_plan(B, H, T, last == 0 ? 0 : std::max<int64_t>(0, T - last), dtype).chunks;
   return chunks == 1 ? 0 : (size_t)chunks * B * H * T * sizeof(float);
 }
 
@@ -340,7 +354,7 @@ extern "C" int kat_attn_key_weights(const void* q, const void* k, const float* L
   a.so[1] = strides[10];
   a.scale = scale;
   a.eps = eps;
-  const KeywPlan p = keyw_plan(B, H, T, a.lo, W, dtype);
+  const KeywPlan p = keyw_plan(B, H, T, a.lo, dtype);
   a.qc = p.qc;
   a.chunks = p.chunks;
   const size_t need = kat_attn_key_weights_workspace_size(B, H, T, D, last, dtype);

@@ -742,15 +742,19 @@ std::optional<Tensor> key_weights(const Tensor& q, const Tensor& k, const Tensor
     return std::nullopt;
   at::NoGradGuard g;
   const c10::DeviceGuard dg(q.device());
-  const Tensor sl = slopes_of(slopes), mask = mask_of(km).t;
+  const Tensor sl = slopes_of(slopes);
+  // the kernels read a bool or byte mask in place; nothing of it is kept
+  const bool as_is = km && (km->scalar_type() == at::kBool || km->scalar_type() == at::kByte) &&
+                     (T <= 1 || km->stride(1) == 1);
+  const Tensor mask = as_is ? *km : mask_of(km).t;
   Tensor w = at::empty({B, H, T}, q.options().dtype(at::kFloat));
   const size_t wsb = kat_attn_key_weights_workspace_size(B, H, T, D, last, code(q));
   const Tensor ws = wsb ? bytes(wsb, q) : Tensor();
   const int64_t s[11] = {q.stride(0), q.stride(1), q.stride(2), k.stride(0), k.stride(1), k.stride(2),
                          L.stride(0), L.stride(1), L.stride(2), w.stride(0), w.stride(1)};
   check(kat_attn_key_weights(q.data_ptr(), k.data_ptr(), L.data_ptr<float>(), w.data_ptr<float>(),
-                             sl.data_ptr<float>(), mask.defined() ? mask.data_ptr<uint8_t>() : nullptr, T,
-                             wsb ? ws.data_ptr() : nullptr, wsb, B, H, T, D, last, s, (float)scale, (float)eps,
+                             sl.data_ptr<float>(), mask.defined() ? static_cast<const uint8_t*>(mask.data_ptr()) : nullptr,
+                             mask.defined() ? mask.stride(0) : 0, wsb ? ws.data_ptr() : nullptr, wsb, B, H, T, D, last, s, (float)scale, (float)eps,
                              code(q), stream(q)),
         "kat_attn_key_weights");
   return w;
