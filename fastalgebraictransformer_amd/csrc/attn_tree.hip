@@ -21,8 +21,8 @@
 //
 // A block streams its rows through LDS in tiles of 64 (LDS-DMA, a ring of
 // NS stages, non-temporal: each row is used once), so rows in flight hold no
-// registers. Its four waves form QG query groups of 16 queries and KG = 4 / QG
-// row groups of a tile:
+// registers. Its waves form QG query groups of 16 queries and KG row groups of a
+// tile:
 //   S^T[row][q] = K Q^T    A = K (LDS rows)             B = Q^T (registers)
 //   f of S^T               lane (g, li) holds rows 4 g + j, query li
 //   O^T[d][q] += V^T f^T   A = V^T (LDS, transposed reads)  B = f packed to the
@@ -64,29 +64,46 @@ struct TreeArgs {
 };
 
 constexpr int kTreeMax = 64;  // tokens: one ancestor mask is one 64-bit word
-constexpr int kTreeWaves = 4;
-constexpr int kTreeRows = 64;  // rows of a tile
+// How a block is laid out, by a row's 16-bit units U and the query groups QG: rows
+// of a tile, waves, stages of the ring (a stage is 4 U bytes per row, of the CU's 160
+// KB of LDS) and blocks per CU. Eight waves run on a CU, in one block where the
+// registers allow it: it then streams one ring four stages deep, and there are half
+// the partial sums (B=8, H=16, N=64, T=8192, D=128: 90 us, against 103 with two
+// blocks of four waves and rings of two stages). At U = 256 eight waves of 64 queries
+// would spill; there, and for 32 queries at U = 128, four waves take tiles of 32 rows (B=4,
+// H=16, N=64, T=2048, D=256 41 us, with 64 43; B=3, H=16, N=25, T=1999, D=96 16.8, with
+// eight waves 19.1). A wave has 16 rows of a tile at least.
+struct TreeShape {
+  int rows, waves, stages, blocks;
+};
+constexpr TreeShape tree_shape(int U, int QG) {
+  return U <= 64 ? TreeShape{64, QG == 1 ? 4 : 8, 4, QG == 1 ? 2 : 1}
+         : QG == 1 ? TreeShape{64, 4, 2, U == 128 ? 2 : 1}
+         : U == 128 && QG == 4 ? TreeShape{64, 8, 4, 1}
+                               : TreeShape{32, 4, 4, U == 128 ? 2 : 1};
+}
+constexpr int tree_qg(int64_t N) { return N <= 16 ? 1 : N <= 32 ? 2 : 4; }
 
-// stages of the ring by a row's 16-bit units: two blocks per CU share 160 KB of
-// LDS up to U = 128 (a stage is 256 U bytes), one at U = 256
-template <int U> constexpr int tree_stages() { return U <= 64 ? 4 : 2; }
+template <typename T, int W, int QG> constexpr TreeShape tree_at() { return tree_shape(W * (int)sizeof(T) / 2, QG); }
 
 template <typename T, int W, int QG, bool POS>
-__global__ __launch_bounds__(64 * kTreeWaves, (W * (int)sizeof(T) > 256 ? 1 : 2)) void attn_tree_k(TreeArgs a) {
+__global__ __launch_bounds__((64 * tree_at<T, W, QG>().waves), (tree_at<T, W, QG>().waves * tree_at<T, W, QG>().blocks / 4))
+void attn_tree_k(TreeArgs a) {
   constexpr int ES = (int)sizeof(T);
   constexpr int U = W * ES / 2;          // a row in 16-bit units, the unit of the tile helpers
   constexpr int KK = U / 32;             // 64-byte column blocks
   constexpr int DS = W / 16;             // 16-wide d subtiles
-  constexpr int TR = kTreeRows, NS = tree_stages<U>();
-  constexpr int KG = kTreeWaves / QG;    // row groups of a tile
+  constexpr TreeShape S = tree_at<T, W, QG>();
+  constexpr int NW = S.waves, TR = S.rows, NS = S.stages;
+  constexpr int KG = NW / QG;            // row groups of a tile
   constexpr int TK = TR / KG;            // rows of a wave's group
-  typedef TileDma<U, kTreeWaves, TR> Dma;
+  typedef TileDma<U, NW, TR> Dma;
   constexpr int OPS = 2 * Dma::SEGS + (POS ? 1 : 0);  // a wave's DMA operations per tile
   constexpr int RING = NS * 2 * TR * U;
-  static_assert(RING * 2 >= kTreeWaves * DS * 1024, "the ring holds the waves' sums");
+  static_assert(TK >= 16 && RING * 2 >= NW * DS * 1024, "the ring holds the waves' sums");
   __shared__ __align__(16) short ring[RING];
-  __shared__ int spos[POS ? NS : 1][kTreeWaves][TR];
-  __shared__ float sl[kTreeWaves][16];
+  __shared__ int spos[POS ? NS : 1][NW][64];  // (a DMA writes 64 words)
+  __shared__ float sl[NW][16];
   __shared__ uint64_t sanc[kTreeMax];  // ancestors of token i, itself included; 0 if absent
   __shared__ int sdep[kTreeMax];       // depth of token i below the context
 
@@ -96,6 +113,20 @@ __global__ __launch_bounds__(64 * kTreeWaves, (W * (int)sizeof(T) > 256 ? 1 : 2)
   const int g = lane >> 4, li = lane & 15;
   const int qg = w % QG, kg = w / QG;
   const int N = a.N;
+  const float slope = a.slopes[h], scale = a.scale;
+  // what does not wait for the length: the queries and the parents
+  const int cols = a.D * ES / 16;  // 16-byte pieces of a row that hold columns
+  const int qi = 16 * qg + li;     // the lane's token
+  i16x8 qf[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) {
+    const int p = 4 * kk + g;
+    qf[kk] = i16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    if (qi < N && p < cols)
+      qf[kk] = *reinterpret_cast<const i16x8*>((const char*)((const T*)a.q + b * a.sq[0] + h * a.sq[1] + qi * a.sq[2]) +
+                                               16 * p);
+  }
+  const int parent = w == 0 && lane < N ? a.parents[b * a.spar + lane] : -2;
   int n = a.lengths ? a.lengths[b] : a.T;
   n = min(n, a.T);
   const int c = n - N;       // rows of the context
@@ -131,7 +162,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, (W * (int)sizeof(T) > 256 ? 1 : 2)
   if (w == 0) {
     // pointer doubling: after step i, anc holds the 2^i nearest ancestors and
     // up the one above them (-1: the context is reached)
-    int up = lane < N ? a.parents[b * a.spar + lane] : -2;
+    int up = parent;
     bool ok = c >= 0 && up >= -1 && up < lane;
     if (!ok) up = -1;
     uint64_t anc = 1ull << lane;
@@ -151,18 +182,6 @@ __global__ __launch_bounds__(64 * kTreeWaves, (W * (int)sizeof(T) > 256 ? 1 : 2)
     sdep[lane] = __popcll(anc) - 1;
   }
 
-  const float slope = a.slopes[h], scale = a.scale;
-  const int cols = a.D * ES / 16;  // 16-byte pieces of a row that hold columns
-  const int qi = 16 * qg + li;     // the lane's token
-  i16x8 qf[KK];
-#pragma unroll
-  for (int kk = 0; kk < KK; ++kk) {
-    const int p = 4 * kk + g;
-    qf[kk] = i16x8{0, 0, 0, 0, 0, 0, 0, 0};
-    if (qi < N && p < cols)
-      qf[kk] = *reinterpret_cast<const i16x8*>((const char*)((const T*)a.q + b * a.sq[0] + h * a.sq[1] + qi * a.sq[2]) +
-                                               16 * p);
-  }
   __syncthreads();  // masks and depths
   const uint64_t anc = qi < N ? sanc[qi] : 0ull;
   int qpos = 0;
@@ -380,15 +399,18 @@ template <typename T, int W> __global__ __launch_bounds__(kTreeCombThreads) void
 // Host side
 // ---------------------------------------------------------------------------
 
-// blocks per (b, h): enough to fill the CUs twice, none without a tile
-static int tree_splits(int64_t B, int64_t H, int64_t T) {
-  const int64_t want = (2 * (int64_t)num_cus() + B * H - 1) / (B * H);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(want, (T + kTreeRows - 1) / kTreeRows));
+// Blocks per (b, h): as many as the CUs hold at once and no more (B=3, H=16, N=25,
+// T=1999, D=96: 8 splits 16.8 us, 12, past what fits, 23.5; 4 splits 20.0), none
+// without a tile.
+static int tree_splits(int64_t B, int64_t H, int64_t N, int64_t T, int W, int dtype) {
+  const TreeShape s = tree_shape(W * dtype_size(dtype) / 2, tree_qg(N));
+  const int64_t want = s.blocks * (int64_t)num_cus() / (B * H);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(want, (T + s.rows - 1) / s.rows));
 }
 
 template <typename T, int W, int QG, bool POS> static int launch_tree(const TreeArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((attn_tree_k<T, W, QG, POS>), dim3((unsigned)a.splits, (unsigned)(a.B * a.H)),
-                     dim3(64 * kTreeWaves), 0, st, a);
+                     dim3(64 * tree_at<T, W, QG>().waves), 0, st, a);
   if (int rc = check_launch("kat_attn_tree")) return rc;
   if (a.splits == 1) return KAT_OK;
   const int64_t rows = (int64_t)a.B * a.H * a.N, rpb = kTreeCombThreads / (W / 4);
@@ -396,18 +418,20 @@ template <typename T, int W, int QG, bool POS> static int launch_tree(const Tree
                      st, a);
   return check_launch("kat_attn_tree (combine)");
 }
-template <typename T, int W> static int tree_qg(const TreeArgs& a, hipStream_t st) {
+template <typename T, int W> static int tree_n(const TreeArgs& a, hipStream_t st) {
   const bool pos = a.positions != nullptr;
-  if (a.N <= 16) return pos ? launch_tree<T, W, 1, true>(a, st) : launch_tree<T, W, 1, false>(a, st);
-  if (a.N <= 32) return pos ? launch_tree<T, W, 2, true>(a, st) : launch_tree<T, W, 2, false>(a, st);
-  return pos ? launch_tree<T, W, 4, true>(a, st) : launch_tree<T, W, 4, false>(a, st);
+  switch (tree_qg(a.N)) {
+    case 1: return pos ? launch_tree<T, W, 1, true>(a, st) : launch_tree<T, W, 1, false>(a, st);
+    case 2: return pos ? launch_tree<T, W, 2, true>(a, st) : launch_tree<T, W, 2, false>(a, st);
+    default: return pos ? launch_tree<T, W, 4, true>(a, st) : launch_tree<T, W, 4, false>(a, st);
+  }
 }
 template <typename T> static int tree_w(const TreeArgs& a, int W, hipStream_t st) {
   switch (W) {
-    case 32: if constexpr (sizeof(T) == 4) return tree_qg<T, 32>(a, st); break;
-    case 64: return tree_qg<T, 64>(a, st);
-    case 128: return tree_qg<T, 128>(a, st);
-    case 256: if constexpr (sizeof(T) == 2) return tree_qg<T, 256>(a, st); break;
+    case 32: if constexpr (sizeof(T) == 4) return tree_n<T, 32>(a, st); break;
+    case 64: return tree_n<T, 64>(a, st);
+    case 128: return tree_n<T, 128>(a, st);
+    case 256: if constexpr (sizeof(T) == 2) return tree_n<T, 256>(a, st); break;
   }
   return fail(KAT_EUNSUPPORTED, "kat_attn_tree: head dim %d", a.D);
 }
@@ -419,7 +443,7 @@ using namespace kat;
 extern "C" size_t kat_attn_tree_workspace_size(int64_t B, int64_t H, int64_t N, int64_t T, int64_t D, int dtype) {
   const int W = cache_layout(D, dtype);
   if (B <= 0 || H <= 0 || T <= 0 || N <= 0 || N > kTreeMax || !W) return 0;
-  const int splits = tree_splits(B, H, T);
+  const int splits = tree_splits(B, H, N, T, W, dtype);
   return splits == 1 ? 0 : (size_t)(B * H) * splits * N * (W + 1) * sizeof(float);
 }
 
@@ -445,7 +469,7 @@ extern "C" int kat_attn_tree(const void* q, const void* k, const void* v, void* 
     return fail(KAT_EUNSUPPORTED, "%s: tensors must be 16-byte aligned", nm);
   if (T > 1 && (strides[5] < D || strides[8] < D)) return fail(KAT_EINVAL, "%s: cache row stride < D", nm);
   // a tile's rows are addressed by 31-bit byte offsets
-  if (T > 1 && std::max(strides[5], strides[8]) > 0x7fffffff / (kTreeRows * esz))
+  if (T > 1 && std::max(strides[5], strides[8]) > 0x7fffffff / (64 * esz))
     return fail(KAT_EUNSUPPORTED, "%s: cache row stride too large", nm);
   TreeArgs a = {};
   a.q = q;
@@ -476,7 +500,7 @@ extern "C" int kat_attn_tree(const void* q, const void* k, const void* v, void* 
   }
   a.scale = scale;
   a.eps = eps;
-  a.splits = tree_splits(B, H, std::max<int64_t>(T, 1));
+  a.splits = tree_splits(B, H, N, std::max<int64_t>(T, 1), W, dtype);
   const size_t need = kat_attn_tree_workspace_size(B, H, N, T, D, dtype);
   if (need && (!workspace || workspace_bytes < need))
     return fail(KAT_EINVAL, "%s: workspace %zu bytes < required %zu", nm, workspace_bytes, need);

@@ -198,6 +198,28 @@ def test_tree_long_cache_splits_and_is_deterministic(gpu):
     check_tree(o, L, q, k, v, slopes, 0.088, parents, None, None)
 
 
+@pytest.mark.parametrize("N", [9, 30, 61])
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float16, 128), (torch.bfloat16, 256),
+                                     (torch.float32, 32), (torch.float32, 64), (torch.float32, 128)])
+def test_tree_of_full_grids(gpu, dtype, D, N):
+    # more heads than blocks fit: one block takes all its tiles, many times round
+    # its ring; three (b, h) checked
+    B, H, T = 33, 16, 700
+    k, v = caches(B, H, T, D, dtype, N)
+    q = rand((B, N, H, D), dtype, N + 2).permute(0, 2, 1, 3)
+    parents = random_parents(B, N, N)
+    lengths = torch.randint(T - 300, T + 1, (B,), generator=torch.Generator().manual_seed(1)).to(torch.int32)
+    slopes = F.compute_alibi_slopes(H)
+    for positions in (None, positions_like(B, H, T, N)):
+        o, L = F.rational_attention_tree(q, k, v, slopes.to(dev), 0.09, parents.to(dev), lengths=lengths.to(dev),
+                                         positions=positions)
+        torch.cuda.synchronize()
+        for b, h in ((0, 0), (17, 5), (B - 1, H - 1)):
+            one = lambda t: t[b:b + 1, h:h + 1]
+            check_tree(one(o), one(L), one(q), one(k), one(v), slopes[h:h + 1], 0.09, parents[b:b + 1],
+                       lengths[b:b + 1], None if positions is None else one(positions))
+
+
 # ------------------------------------------------------------- accumulate ----
 
 def check_accumulate(o, L, total, old, q, k, v, slopes, scale, lengths, positions):
