@@ -8,15 +8,19 @@
 //   L = sum_j f_j,  o = sum_j f_j v_j / (L + eps)
 //   total_j += f_j / (L + eps)   (j < n)
 //
-// Design: the decode's split over the rows (HBM bounds it: 2 D dtype bytes per
-// row, and 16 bytes for the totals and the f between the two launches). L is
-// known only after every chunk, so the chunks also leave their f in the
-// workspace, and the second kernel, which adds the chunks' sums, adds f / (L +
-// eps) to the totals in blocks beside those that write o. The chunks are sized
-// by the rows that are filled, so a short sequence in a long cache spreads over
-// all blocks. No atomics: every total belongs to one thread.
+// Design: HBM bounds it (2 D dtype bytes per row and 8 for its total). Where the
+// (b, h) fill the chip, or their rows are few, a block takes all rows of one, keeps
+// the f in LDS and finishes o, L and the totals itself. Else the decode's split over
+// the rows: L is known only after every chunk, so the chunks leave their f in the
+// workspace (8 more bytes per row), and the second kernel, which adds the chunks'
+// sums, adds f / (L + eps) to the totals in blocks beside those that write o. The
+// chunks are sized by the rows that are filled, so a short sequence in a long cache
+// spreads over all blocks. No atomics: every total belongs to one thread.
+// B=16, H=16, T=4096, D=128, bf16: 86 us = 6.3 TB/s; four scores per lane instead of
+// one, with a load per position and a store per f of each, took 105 us.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_cache.h"
 #include "kat_internal.h"
@@ -48,13 +52,14 @@ constexpr int kAccThreads = 256;
 constexpr int kAccWaves = kAccThreads / 64;
 constexpr int kAccInFlight = 4;  // rows per lane in flight
 constexpr int kAccRowsPerBlock = 4 * kAccThreads;  // totals per block of the second kernel
+constexpr int kOneWaves = 16;    // one launch: waves of the block of a (b, h)
+constexpr int kOneRows = 8192;   // most rows of it (their f stay in LDS)
 
 template <typename T, int W> struct AccShape {
   static constexpr int EPL = 16 / (int)sizeof(T);     // elements per lane
   static constexpr int LPR = W / EPL;                 // lanes per row
   static constexpr int RPW = 64 / LPR;                // rows per wave per load
   static constexpr int RPI = RPW * kAccInFlight;      // consecutive rows per wave per pass
-  static constexpr int RPP = RPI * kAccWaves;         // rows per block per pass
   static_assert(LPR >= 4 && LPR <= 64, "a row is at least a quad of lanes");
 };
 
@@ -69,20 +74,25 @@ template <int CTRL> __device__ __forceinline__ float quad(float x) {
 // quad halve the values at every step, then one sum per further step): each lane
 // maps one score instead of four, loads one position and the first quad of a row
 // stores one f.
-template <typename T, int W, bool POS>
-__global__ __launch_bounds__(kAccThreads) void attn_accum_part_k(AccumArgs a) {
+// ONE: the block takes all rows of its (b, h) and writes o, L and the totals itself.
+template <typename T, int W, bool POS, bool ONE>
+__global__ __launch_bounds__(64 * (ONE ? kOneWaves : kAccWaves)) void attn_accum_part_k(AccumArgs a) {
   typedef AccShape<T, W> S;
-  constexpr int EPL = S::EPL, LPR = S::LPR, RPW = S::RPW, RPI = S::RPI, RPP = S::RPP, U = kAccInFlight;
+  constexpr int EPL = S::EPL, LPR = S::LPR, RPW = S::RPW, RPI = S::RPI, U = kAccInFlight;
+  constexpr int NW = ONE ? kOneWaves : kAccWaves, NT = 64 * NW;
+  constexpr int RPP = RPI * NW;  // rows per block per pass
   static_assert(U == 4, "a load per lane of a quad");
-  __shared__ float sh_acc[kAccWaves][W];
-  __shared__ float sh_l[kAccWaves];
+  __shared__ float sh_acc[NW][W];
+  __shared__ float sh_l[NW];
+  __shared__ float sh_f[ONE ? kOneRows : 1];
   const int bh = blockIdx.y, b = bh / a.H, h = bh - b * a.H;
   const int split = blockIdx.x;
   const int lane = threadIdx.x & 63, w = wave_id();
   const int sub = lane % LPR, grp = lane / LPR, qd = lane & 3;
   int n = a.lengths ? a.lengths[b] : a.T;
   n = min(max(n, 0), a.T);  // a bad length cannot move a read out of the cache
-  const int per = ((n + RPP - 1) / RPP + a.splits - 1) / a.splits * RPP;
+  const int splits = ONE ? 1 : a.splits;
+  const int per = ((n + RPP - 1) / RPP + splits - 1) / splits * RPP;
   const int j0 = split * per, j1 = min(j0 + per, n);
   const float slope = a.slopes[h];
   const int32_t* pp = POS ? a.positions + b * a.spos[0] + h * a.spos[1] : nullptr;
@@ -127,7 +137,10 @@ __global__ __launch_bounds__(kAccThreads) void attn_accum_part_k(AccumArgs a) {
     for (int off = 4; off < LPR; off <<= 1) s += __shfl_xor(s, off, 64);
     const float t = sig2_pow4(s - slope * (float)(qpos - pos));
     const float f = mine < j1 ? t : 0.f;
-    if (sub < 4 && mine < j1) fp[mine] = f;
+    if (sub < 4 && mine < j1) {
+      if constexpr (ONE) sh_f[mine] = f;
+      else fp[mine] = f;
+    }
     l += f;
     const float fu[U] = {quad<0x00>(f), quad<0x55>(f), quad<0xAA>(f), quad<0xFF>(f)};
 #pragma unroll
@@ -149,14 +162,36 @@ __global__ __launch_bounds__(kAccThreads) void attn_accum_part_k(AccumArgs a) {
     for (int e = 0; e < EPL; ++e) sh_acc[w][sub * EPL + e] = acc[e];
     if (sub == 0) sh_l[w] = l;
   }
-  __syncthreads();
-  const int64_t p = (int64_t)bh * a.splits + split;
-  for (int d = threadIdx.x; d <= W; d += kAccThreads) {
-    float t = 0.f;
+  if constexpr (ONE) {
+    // the totals' loads run beside the exchange
+    float* tp = a.total + b * a.stot[0] + h * a.stot[1];
+    float old = (int)threadIdx.x < n ? tp[threadIdx.x] : 0.f;
+    __syncthreads();
+    l = 0.f;
 #pragma unroll
-    for (int ww = 0; ww < kAccWaves; ++ww) t += d < W ? sh_acc[ww][d] : sh_l[ww];
-    if (d < W) a.part[p * W + d] = t;
-    else a.lpart[p] = t;
+    for (int ww = 0; ww < NW; ++ww) l += sh_l[ww];
+    const float inv = 1.f / (l + 16.f * a.eps);
+    if (threadIdx.x == 0 && a.L) a.L[bh] = l * 0.0625f;
+    if ((int)threadIdx.x < a.D) {
+      float t = 0.f;
+#pragma unroll
+      for (int ww = 0; ww < NW; ++ww) t += sh_acc[ww][threadIdx.x];
+      ((T*)a.o)[b * a.so[0] + h * a.so[1] + threadIdx.x] = from_acc<T>(t * inv);
+    }
+    for (int j = threadIdx.x; j < n; j += NT) {
+      if (j >= NT) old = tp[j];
+      tp[j] = fmaf(sh_f[j], inv, old);
+    }
+  } else {
+    __syncthreads();
+    const int64_t p = (int64_t)bh * a.splits + split;
+    for (int d = threadIdx.x; d <= W; d += NT) {
+      float t = 0.f;
+#pragma unroll
+      for (int ww = 0; ww < NW; ++ww) t += d < W ? sh_acc[ww][d] : sh_l[ww];
+      if (d < W) a.part[p * W + d] = t;
+      else a.lpart[p] = t;
+    }
   }
 }
 
@@ -224,6 +259,19 @@ template <typename T, int W> __global__ __launch_bounds__(kAccThreads) void attn
 
 static int accum_rpp(int W, int dtype) { return 64 / (W * dtype_size(dtype) / 16) * kAccInFlight * kAccWaves; }
 
+// One launch, a block of 16 waves per (b, h): saves the second launch and the f in
+// memory, but a CU streams no more than some 35 GB/s into one block. Taken where the
+// (b, h) fill half the CUs, or their rows take less than the second launch: with c =
+// 0.56 CUs, bytes per (b, h) x (c - BH) below 20 MB (rates of 35 kB/us per block and
+// 5 MB/us in all, 4 us for the launch). bf16, two launches / one, us: 12 heads of 64, T=576
+// 7.0 / 4.8; 96 heads, T=1152 11.9 / 10.7, T=2304 16.8 / 19.6; 16 heads of 128, T=1000 6.4
+// / 13.0; 256 heads of 128, T=1024 27.6 / 23.6, T=4096 94.2 / 86.5; 384 of 64, T=2304
+// 43 / 44; fp32, 48 heads of 64, T=512 7.0 / 8.7.
+static bool accum_one(int64_t B, int64_t H, int64_t T, int W, int dtype) {
+  const double row = 2.0 * W * dtype_size(dtype);
+  return T <= kOneRows && row * T * (0.56 * num_cus() - (double)(B * H)) < 20e6;
+}
+
 // chunks per (b, h): three blocks per CU, none smaller than one block pass (1 / 2 / 3 /
 // 4 blocks: B=16, H=16, T=4096, D=128 110 / 98 / 96 / 100 us, B=4, H=12, T=2048, D=64 in
 // fp32 16.6 / 14.1 / 12.5 / 14.7)
@@ -232,23 +280,29 @@ static int accum_splits(int64_t B, int64_t H, int64_t T, int W, int dtype) {
   return (int)std::max<int64_t>(1, std::min(want, (T + rpp - 1) / rpp));
 }
 
-template <typename T, int W> static int launch_accum(const AccumArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)a.splits, (unsigned)(a.B * a.H));
-  if (a.positions)
-    hipLaunchKernelGGL((attn_accum_part_k<T, W, true>), grid, dim3(kAccThreads), 0, st, a);
-  else
-    hipLaunchKernelGGL((attn_accum_part_k<T, W, false>), grid, dim3(kAccThreads), 0, st, a);
+template <typename T, int W, bool POS> static int launch_accum(const AccumArgs& a, bool one, hipStream_t st) {
+  if (one) {
+    hipLaunchKernelGGL((attn_accum_part_k<T, W, POS, true>), dim3(1, (unsigned)(a.B * a.H)), dim3(64 * kOneWaves), 0, st, a);
+    return check_launch("kat_attn_decode_accum");
+  }
+  hipLaunchKernelGGL((attn_accum_part_k<T, W, POS, false>), dim3((unsigned)a.splits, (unsigned)(a.B * a.H)),
+                     dim3(kAccThreads), 0, st, a);
   if (int rc = check_launch("kat_attn_decode_accum (partials)")) return rc;
   const unsigned nb = 1 + (unsigned)((a.T + kAccRowsPerBlock - 1) / kAccRowsPerBlock);
   hipLaunchKernelGGL((attn_accum_finish_k<T, W>), dim3(nb, (unsigned)(a.B * a.H)), dim3(kAccThreads), 0, st, a);
   return check_launch("kat_attn_decode_accum (totals)");
 }
 template <typename T> static int accum_w(const AccumArgs& a, int W, hipStream_t st) {
+  const bool one = accum_one(a.B, a.H, a.T, W, sizeof(T) == 4 ? KAT_F32 : KAT_BF16);
+  auto go = [&](auto w) {
+    constexpr int kW = decltype(w)::value;
+    return a.positions ? launch_accum<T, kW, true>(a, one, st) : launch_accum<T, kW, false>(a, one, st);
+  };
   switch (W) {
-    case 32: if constexpr (sizeof(T) == 4) return launch_accum<T, 32>(a, st); break;
-    case 64: return launch_accum<T, 64>(a, st);
-    case 128: return launch_accum<T, 128>(a, st);
-    case 256: if constexpr (sizeof(T) == 2) return launch_accum<T, 256>(a, st); break;
+    case 32: if constexpr (sizeof(T) == 4) return go(std::integral_constant<int, 32>{}); break;
+    case 64: return go(std::integral_constant<int, 64>{});
+    case 128: return go(std::integral_constant<int, 128>{});
+    case 256: if constexpr (sizeof(T) == 2) return go(std::integral_constant<int, 256>{}); break;
   }
   return fail(KAT_EUNSUPPORTED, "kat_attn_decode_accum: head dim %d", a.D);
 }
@@ -259,7 +313,7 @@ using namespace kat;
 
 extern "C" size_t kat_attn_decode_accum_workspace_size(int64_t B, int64_t H, int64_t T, int64_t D, int dtype) {
   const int W = cache_layout(D, dtype);
-  if (B <= 0 || H <= 0 || T <= 0 || !W) return 0;
+  if (B <= 0 || H <= 0 || T <= 0 || !W || accum_one(B, H, T, W, dtype)) return 0;
   return (size_t)(B * H) * ((size_t)accum_splits(B, H, T, W, dtype) * (W + 1) + T) * sizeof(float);
 }
 
@@ -311,7 +365,7 @@ extern "C" int kat_attn_decode_accum(const void* q, const void* k, const void* v
   a.eps = eps;
   a.splits = accum_splits(B, H, std::max<int64_t>(T, 1), W, dtype);
   const size_t need = kat_attn_decode_accum_workspace_size(B, H, std::max<int64_t>(T, 1), D, dtype);
-  if (!workspace || workspace_bytes < need)
+  if (need && (!workspace || workspace_bytes < need))
     return fail(KAT_EINVAL, "%s: workspace %zu bytes < required %zu", nm, workspace_bytes, need);
   a.part = (float*)workspace;
   a.lpart = a.part + (size_t)(B * H) * a.splits * W;

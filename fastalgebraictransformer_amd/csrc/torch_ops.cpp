@@ -671,7 +671,7 @@ std::optional<std::tuple<Tensor, Tensor>> tree(const Tensor& q, const Tensor& k,
                                                const std::optional<Tensor>& positions, double eps) {
   if (q.dim() != 4 || !cache_ok(q, k, v, slopes)) return std::nullopt;
   const int64_t B = q.size(0), H = q.size(1), N = q.size(2), D = q.size(3), T = k.size(2);
-  if (!ints(q, parents) || parents.dim() < 1 || parents.dim() > 2 || parents.size(-1) != N ||
+  if (N > 64 || !ints(q, parents) || parents.dim() < 1 || parents.dim() > 2 || parents.size(-1) != N ||
       (parents.dim() == 2 && parents.size(0) != B) || (N > 1 && parents.stride(-1) != 1) ||
       !lengths_ok(q, lengths, B) || !positions_ok(q, positions, B, H, T))
     return std::nullopt;
@@ -718,7 +718,7 @@ std::optional<std::tuple<Tensor, Tensor>> decode_accumulate(const Tensor& q, con
   Tensor out = at::empty({B, H, D}, q.options().memory_format(at::MemoryFormat::Contiguous));
   Tensor L = at::empty({B, H}, q.options().dtype(at::kFloat));
   const size_t wsb = kat_attn_decode_accum_workspace_size(B, H, T, D, code(q));
-  const Tensor ws = bytes(wsb, q);
+  const Tensor ws = wsb ? bytes(wsb, q) : Tensor();
   const int64_t s[10] = {q.stride(0), q.stride(1), k.stride(0), k.stride(1), k.stride(2),
                          v.stride(0), v.stride(1), v.stride(2), out.stride(0), out.stride(1)};
   const int64_t wp[4] = {weights.stride(0), weights.stride(1), positions ? positions->stride(0) : 0,
@@ -726,8 +726,8 @@ std::optional<std::tuple<Tensor, Tensor>> decode_accumulate(const Tensor& q, con
   check(kat_attn_decode_accum(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), L.data_ptr<float>(),
                               sl.data_ptr<float>(), weights.data_ptr<float>(),
                               lengths ? lengths->data_ptr<int32_t>() : nullptr,
-                              positions ? positions->data_ptr<int32_t>() : nullptr, wp, ws.data_ptr(), wsb, B, H, T, D,
-                              s, (float)scale, (float)eps, code(q), stream(q)),
+                              positions ? positions->data_ptr<int32_t>() : nullptr, wp, wsb ? ws.data_ptr() : nullptr, wsb,
+                              B, H, T, D, s, (float)scale, (float)eps, code(q), stream(q)),
         "kat_attn_decode_accum");
   return std::make_tuple(out, L);
 }
@@ -735,7 +735,7 @@ std::optional<std::tuple<Tensor, Tensor>> decode_accumulate(const Tensor& q, con
 // q, k [B, H, T, D], L [B, H, T]: weights [B, H, T]; last == 0: every query
 std::optional<Tensor> key_weights(const Tensor& q, const Tensor& k, const Tensor& slopes, double scale, const Tensor& L,
                                   const std::optional<Tensor>& km, int64_t last, double eps) {
-  if (q.dim() != 4 || !cache_ok(q, k, k, slopes) || k.sizes() != q.sizes()) return std::nullopt;
+  if (q.dim() != 4 || last < 0 || !cache_ok(q, k, k, slopes) || k.sizes() != q.sizes()) return std::nullopt;
   const int64_t B = q.size(0), H = q.size(1), T = q.size(2), D = q.size(3);
   if (!same_place(q, {&L}) || L.scalar_type() != at::kFloat || L.dim() != 3 || L.sizes() != q.sizes().slice(0, 3) ||
       !mask_ok(q, km, B, T))

@@ -86,15 +86,15 @@ def rational_attention_tree(q, k_cache, v_cache, alibi_slopes, scale, parents, l
 
     Returns (out [B, H, N, D] in q's dtype and row order, L [B, H, N] fp32
     without eps). With N = 1 and parents -1 it is rational_attention_decode."""
+    r = _lib.ops().tree(q, k_cache, v_cache, alibi_slopes, scale, parents, lengths, positions, eps)
+    if r is not None:
+        return r
     assert q.is_cuda and k_cache.is_cuda and v_cache.is_cuda
     B, H, N, D = q.shape
     T = k_cache.shape[2]
     assert tuple(k_cache.shape) == (B, H, T, D) and tuple(v_cache.shape) == (B, H, T, D)
     assert N <= MAX_TREE, f"at most {MAX_TREE} drafted tokens"
     assert tuple(parents.shape) in ((N,), (B, N)), f"parents must be [N] or [B, N] = [{B}, {N}]"
-    r = _lib.ops().tree(q, k_cache, v_cache, alibi_slopes, scale, parents, lengths, positions, eps)
-    if r is not None:
-        return r
     lib = _lib.load()
     q, k, v = _unit_d(q), _unit_d(k_cache.to(q.dtype)), _unit_d(v_cache.to(q.dtype))
     slopes = _slopes_arg(alibi_slopes, q)
@@ -128,14 +128,14 @@ def rational_attention_decode_accumulate(q, k_cache, v_cache, alibi_slopes, scal
     positions[lengths[b] - 1] - positions[j], for caches whose rows have been
     evicted; without, rows are positions. Other arguments, types and head dims
     as rational_attention_decode. Returns (out [B, H, D], L [B, H])."""
-    assert q.is_cuda and k_cache.is_cuda and v_cache.is_cuda
-    B, H, D = q.shape
-    T = k_cache.shape[2]
-    assert tuple(k_cache.shape) == (B, H, T, D) and tuple(v_cache.shape) == (B, H, T, D)
     r = _lib.ops().decode_accumulate(q, k_cache, v_cache, alibi_slopes, scale, weights, lengths,
                                      positions, eps)
     if r is not None:
         return r
+    assert q.is_cuda and k_cache.is_cuda and v_cache.is_cuda
+    B, H, D = q.shape
+    T = k_cache.shape[2]
+    assert tuple(k_cache.shape) == (B, H, T, D) and tuple(v_cache.shape) == (B, H, T, D)
     _check_rows("weights", weights, (B, H, T), torch.float32, q.device)
     lib = _lib.load()
     q, k, v = _unit_d(q), _unit_d(k_cache.to(q.dtype)), _unit_d(v_cache.to(q.dtype))
@@ -170,15 +170,15 @@ def rational_attention_key_weights(q, k, alibi_slopes, scale, L, key_mask=None, 
     queries count (default all). ``key_mask`` ([B, T], 0 drops a token): a
     dropped token neither gives nor receives weight; L is then the masked
     attention's."""
-    assert q.is_cuda and k.is_cuda and L.is_cuda
-    assert q.shape == k.shape and tuple(L.shape) == tuple(q.shape[:3])
-    B, H, T, D = q.shape
     assert last is None or last >= 1, "last must be at least 1"
-    assert key_mask is None or tuple(key_mask.shape) == (B, T), f"key_mask must be [B, T] = [{B}, {T}]"
-    n = 0 if last is None or last >= T else int(last)
+    n = 0 if last is None else min(int(last), 1 << 40)
     r = _lib.ops().key_weights(q, k, alibi_slopes, scale, L, key_mask, n, eps)
     if r is not None:
         return r
+    assert q.is_cuda and k.is_cuda and L.is_cuda
+    assert q.shape == k.shape and tuple(L.shape) == tuple(q.shape[:3])
+    B, H, T, D = q.shape
+    assert key_mask is None or tuple(key_mask.shape) == (B, T), f"key_mask must be [B, T] = [{B}, {T}]"
     lib = _lib.load()
     q, k = _unit_d(q), _unit_d(k.to(q.dtype))
     L = L.to(device=q.device, dtype=torch.float32)
@@ -212,13 +212,13 @@ def kv_cache_evict(k_cache, v_cache, weights, positions, lengths, keep, recent=0
     the inputs stay as they are (out's ``lengths`` too is another tensor than the
     one given); rows behind them are left alone.
     Returns the five tensors that hold the result."""
-    assert k_cache.is_cuda and v_cache.is_cuda
     if out is not None:
         out = tuple(out)
         assert len(out) == 5, "out must be (k, v, weights, positions, lengths)"
     res = (k_cache, v_cache, weights, positions, lengths) if out is None else out
     if _lib.ops().evict(k_cache, v_cache, weights, positions, lengths, out, keep, recent):
         return res
+    assert k_cache.is_cuda and v_cache.is_cuda
     B, H, T, D = k_cache.shape
     assert tuple(v_cache.shape) == (B, H, T, D) and v_cache.dtype == k_cache.dtype
     assert 0 <= recent <= keep, "recent must lie in [0, keep]"

@@ -314,7 +314,8 @@ int kat_attn_tree(const void* q, const void* k, const void* v, void* out, float*
  * distance of row j is positions[n - 1] - positions[j] instead of n - 1 - j: a
  * cache whose rows have been evicted. wp_strides: 4 int64 = (b, h) of weights
  * and of positions, unit t-stride; weights must not overlap themselves. Other
- * arguments as kat_attn_decode. No counterpart in the reference. */
+ * arguments as kat_attn_decode; the workspace may be NULL where its size is 0. No
+ * counterpart in the reference. */
 size_t kat_attn_decode_accum_workspace_size(int64_t B, int64_t H, int64_t T, int64_t D, int dtype);
 int kat_attn_decode_accum(const void* q, const void* k, const void* v, void* out, float* L,
                           const float* slopes, float* weights, const int32_t* lengths,

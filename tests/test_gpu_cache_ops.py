@@ -262,6 +262,46 @@ def test_accumulate_matches_definition(gpu, dtype, D, n):
         assert torch.equal(buf, old)  # nothing outside the view
 
 
+@pytest.mark.parametrize("n", [1, 31, 129])
+@pytest.mark.parametrize("dtype,D", DIMS)
+def test_accumulate_of_few_rows(gpu, dtype, D, n):
+    # a block per (b, h), which finishes its totals itself
+    B, H, T = 3, 2, 130
+    k, v = caches(B, H, T, D, dtype, n + D)
+    q = rand((B, H, D), dtype, n + D + 2)
+    lengths = torch.tensor([n, 0, T + 5], dtype=torch.int32)
+    slopes = F.compute_alibi_slopes(H)
+    for positions in (None, positions_like(B, H, T, n)):
+        total = torch.rand(B, H, T, generator=torch.Generator().manual_seed(n)).to(dev)
+        old = total.clone()
+        o, L = F.rational_attention_decode_accumulate(q, k, v, slopes.to(dev), 0.1, total,
+                                                      lengths=lengths.to(dev), positions=positions)
+        torch.cuda.synchronize()
+        check_accumulate(o, L, total, old, q, k, v, slopes, 0.1, lengths, positions)
+
+
+@pytest.mark.parametrize("dtype,D,T", [(torch.bfloat16, 64, 700), (torch.float16, 256, 300), (torch.float32, 128, 300),
+                                       (torch.float16, 8, 8192), (torch.float16, 8, 8193)])
+def test_accumulate_of_full_grids(gpu, dtype, D, T):
+    # more heads than CUs: a block per (b, h) up to 8192 rows, chunks beyond; three
+    # (b, h) checked
+    B, H = 33, 16
+    k, v = caches(B, H, T, D, dtype, T)
+    q = rand((B, H, D), dtype, T + 2)
+    lengths = torch.randint(T // 2, T + 1, (B,), generator=torch.Generator().manual_seed(1)).to(torch.int32)
+    lengths[0] = T
+    slopes = F.compute_alibi_slopes(H)
+    total = torch.rand(B, H, T, generator=torch.Generator().manual_seed(T)).to(dev)
+    old, positions = total.clone(), positions_like(B, H, T, T)
+    o, L = F.rational_attention_decode_accumulate(q, k, v, slopes.to(dev), 0.1, total, lengths=lengths.to(dev),
+                                                  positions=positions)
+    torch.cuda.synchronize()
+    for b, h in ((0, 0), (17, 5), (B - 1, H - 1)):
+        one = lambda t: t[b:b + 1, h:h + 1]
+        check_accumulate(one(o), one(L), one(total), one(old), one(q), one(k), one(v), slopes[h:h + 1], 0.1,
+                         lengths[b:b + 1], one(positions))
+
+
 def test_accumulate_agrees_with_decode_and_adds_up(gpu):
     B, H, T, D = 2, 4, 2000, 64
     k, v = caches(B, H, T, D, torch.bfloat16, 21)

@@ -63,7 +63,10 @@ def test_accumulate_refusals():
     assert call(weights=None) == 1 and call(wp=False) == 1 and "null" in _msg()
     assert call(T=-1) == 1 and call(T=1 << 30) == 2
     assert call(strides=[64] * 4 + [8] + [64] * 5) == 1 and "row stride" in _msg()
-    assert call() == 1 and "workspace 0 bytes" in _msg()
+    # few rows take one launch and no workspace, a long cache of few heads does
+    assert lib.kat_attn_decode_accum_workspace_size(1, 2, 9, 64, 1) == 0
+    assert lib.kat_attn_decode_accum_workspace_size(1, 2, 5000, 64, 1) > 2 * 5000 * 4
+    assert call(T=5000) == 1 and "workspace 0 bytes" in _msg()
 
 
 def test_key_weights_refusals():
