@@ -18,9 +18,11 @@ import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint
 
 from .backward import attention_torch, rational_attention_packed
-from .forward import compute_alibi_slopes, rational_attention_decode
+from .forward import _attn_fwd_into, compute_alibi_slopes, rational_attention_decode
 from .fused_ops import (EPS, add_mean_error_norm, mean_error_norm, rational_softmax,
                         rational_swiglu_packed)
+from .kv_cache import (kv_cache_evict, rational_attention_decode_accumulate,
+                       rational_attention_key_weights, rational_attention_tree)
 
 
 def _narrow(x: torch.Tensor) -> Optional[torch.dtype]:
@@ -38,12 +40,59 @@ class KVCache:
     """Keys and values of one block for cached decoding: [batch, max_len,
     n_head, d_head] each (token-major, as the qkv projection lays them out),
     allocated on first use in the dtype the projection produces (bf16 under
-    autocast)."""
+    autocast).
 
-    def __init__(self, max_len: int):
+    With ``keep`` the cache is bounded: it also holds, [batch, n_head, max_len]
+    each, the attention weight every key has received (fp32) and its position
+    (int32), and evict() leaves the ``keep`` keys with the largest weights, the
+    ``recent`` newest always among them."""
+
+    def __init__(self, max_len: int, keep: Optional[int] = None, recent: int = 0):
+        assert keep is None or 0 <= recent <= keep < max_len, "need recent <= keep < max_len"
         self.max_len = max_len
+        self.keep, self.recent = keep, recent
         self.k: Optional[torch.Tensor] = None
         self.v: Optional[torch.Tensor] = None
+        self.weights: Optional[torch.Tensor] = None
+        self.positions: Optional[torch.Tensor] = None
+        self.lengths: Optional[torch.Tensor] = None
+
+    def allocate(self, like: torch.Tensor):
+        """Buffers for keys like ``like`` [batch, tokens, n_head, d_head]."""
+        B, _, H, D = like.shape
+        self.k = torch.empty((B, self.max_len, H, D), dtype=like.dtype, device=like.device)
+        self.v = torch.empty_like(self.k)
+        if self.keep is not None:
+            self.weights = torch.zeros((B, H, self.max_len), device=like.device)
+            self.positions = torch.zeros((B, H, self.max_len), dtype=torch.int32, device=like.device)
+            self.lengths = torch.zeros(B, dtype=torch.int32, device=like.device)
+
+    def _rows(self):
+        return (self.k.permute(0, 2, 1, 3), self.v.permute(0, 2, 1, 3), self.weights, self.positions,
+                self.lengths)
+
+    def fill(self, k: torch.Tensor, v: torch.Tensor, weights: torch.Tensor):
+        """The keys and values of a prompt ([batch, n_head, tokens, d_head]) with
+        the weight each key received, down to ``keep`` of them."""
+        B, H, T, _ = k.shape
+        at = torch.arange(T, dtype=torch.int32, device=k.device).expand(B, H, T)
+        kv_cache_evict(k, v, weights, at, None, self.keep, self.recent, out=self._rows())
+
+    def evict(self, n: int):
+        """From ``n`` filled rows down to ``keep``."""
+        self.lengths.fill_(n)
+        k, v, w, p, lengths = self._rows()
+        kv_cache_evict(k, v, w, p, lengths, self.keep, self.recent)
+
+    def accept(self, n: int, path: torch.Tensor):
+        """The rows n + path[b, j] of drafted tokens to rows n + j (path: int64
+        [batch, m], ascending); rows behind are free again."""
+        m = path.size(1)
+        for t, dim in ((self.k, 1), (self.v, 1), (self.positions, 2)):
+            if t is not None:
+                at = (path + n).view([path.size(0)] + [m if d == dim else 1 for d in range(1, t.dim())])
+                shape = [m if d == dim else size for d, size in enumerate(t.shape)]
+                t.narrow(dim, n, m).copy_(t.gather(dim, at.expand(shape)))
 
 
 class RationalMR(nn.Module):
@@ -117,9 +166,11 @@ class AlgebraicAttention(nn.Module):
         B, T, C = x.shape
         qkv = self.qkv(x).view(B, T, 3, self.n_head, self.d_head)
         if cache.k is None:
-            shape = (B, cache.max_len, self.n_head, self.d_head)
-            cache.k = torch.empty(shape, dtype=qkv.dtype, device=qkv.device)
-            cache.v = torch.empty(shape, dtype=qkv.dtype, device=qkv.device)
+            cache.allocate(qkv[:, :, 1])
+        if cache.keep is not None:
+            assert pos0 == 0, "tokens after the prompt are decoded (decode_step)"
+            y = self._prompt_bounded(qkv, cache)
+            return self.dropout(self.out(y.view(B, T, C)))
         assert pos0 + T <= cache.max_len, "KV cache is full"
         kc, vc = cache.k, cache.v
         kc[:, pos0:pos0 + T] = qkv[:, :, 1]
@@ -135,18 +186,59 @@ class AlgebraicAttention(nn.Module):
             y = y.reshape(B, 1, C)
         return self.dropout(self.out(y))
 
+    def _prompt_bounded(self, qkv: torch.Tensor, cache: KVCache) -> torch.Tensor:
+        """Causal attention of a prompt whose keys go into a bounded cache by
+        the weight that all of its queries give them."""
+        B, T, _, H, D = qkv.shape
+        q, k, v = qkv.permute(2, 0, 3, 1, 4)
+        y = torch.empty((B, T, H, D), dtype=qkv.dtype, device=qkv.device)
+        L = torch.empty((B, H, T), dtype=torch.float32, device=qkv.device)
+        _attn_fwd_into(q, k, v, y.permute(0, 2, 1, 3), L, self.alibi_slopes, self.scale, True, EPS)
+        w = rational_attention_key_weights(q, k, self.alibi_slopes, self.scale, L, eps=EPS)
+        cache.fill(k, v, w)
+        return y
+
+    def forward_tree(self, x: torch.Tensor, cache: KVCache, parents: torch.Tensor, n: int,
+                     lengths: torch.Tensor, positions: Optional[torch.Tensor]) -> torch.Tensor:
+        """Drafted tokens x [B, N, C] over ``n`` cached rows, each attending to
+        them and to its ancestors (``parents``, see rational_attention_tree);
+        their keys and values go into rows n .. n + N - 1. ``lengths`` = n + N
+        (int32 [B]); ``positions`` (int32 [B, N]): theirs, for a bounded cache."""
+        B, N, C = x.shape
+        qkv = self.qkv(x).view(B, N, 3, self.n_head, self.d_head)
+        assert n + N <= cache.max_len, "KV cache is full"
+        cache.k[:, n:n + N] = qkv[:, :, 1]
+        cache.v[:, n:n + N] = qkv[:, :, 2]
+        if cache.keep is not None:
+            cache.weights[:, :, n:n + N] = 0.0
+            cache.positions[:, :, n:n + N] = positions[:, None]
+        y, _ = rational_attention_tree(qkv[:, :, 0].permute(0, 2, 1, 3), cache.k.permute(0, 2, 1, 3),
+                                       cache.v.permute(0, 2, 1, 3), self.alibi_slopes, self.scale,
+                                       parents, lengths=lengths, positions=cache.positions, eps=EPS)
+        return self.dropout(self.out(y.transpose(1, 2).reshape(B, N, C)))
+
     def decode_step(self, x: torch.Tensor, cache: KVCache, pos: torch.Tensor,
-                    lengths: torch.Tensor) -> torch.Tensor:
+                    lengths: torch.Tensor, position: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One new token per batch row (x: [B, 1, C]) at the position held on the
         device in ``pos`` (int64 [1]), with ``lengths`` = pos + 1 (int32 [B]):
         its key and value go into the cache at ``pos`` and the decode kernel
         attends over the first ``lengths`` cached positions. No host-side
         position enters the computation, so the step can be captured in a
-        HIP graph and replayed for every token."""
+        HIP graph and replayed for every token. In a bounded cache ``pos`` is the
+        row, ``position`` (int32 [1]) the token's position, and the keys' weights
+        grow by this token's."""
         B, T, C = x.shape
         qkv = self.qkv(x).view(B, 1, 3, self.n_head, self.d_head)
         cache.k.index_copy_(1, pos, qkv[:, :, 1])
         cache.v.index_copy_(1, pos, qkv[:, :, 2])
+        if cache.keep is not None:
+            cache.weights.index_fill_(2, pos, 0.0)
+            cache.positions.index_copy_(2, pos, position.expand(B, self.n_head, 1))
+            y, _ = rational_attention_decode_accumulate(
+                qkv[:, 0, 0], cache.k.permute(0, 2, 1, 3), cache.v.permute(0, 2, 1, 3),
+                self.alibi_slopes, self.scale, cache.weights, lengths=lengths,
+                positions=cache.positions, eps=EPS)
+            return self.dropout(self.out(y.reshape(B, 1, C)))
         y, _ = rational_attention_decode(qkv[:, 0, 0], cache.k.permute(0, 2, 1, 3),
                                          cache.v.permute(0, 2, 1, 3), self.alibi_slopes,
                                          self.scale, lengths=lengths, eps=EPS)
@@ -187,13 +279,23 @@ class AlgebraicBlock(nn.Module):
         return h, self.ffn(n2)
 
     def decode_pending(self, x: torch.Tensor, r: Optional[torch.Tensor], cache, pos: torch.Tensor,
-                       lengths: torch.Tensor):
+                       lengths: torch.Tensor, position: Optional[torch.Tensor] = None):
         """forward_pending for one new token (AlgebraicAttention.decode_step)."""
         if r is None:
             h0, n1 = x, self.norm1(x)
         else:
             h0, n1 = add_mean_error_norm(x, r, self.norm1.weight, self.norm1.eps, _narrow(x))
-        h, n2 = add_mean_error_norm(h0, self.attn.decode_step(n1, cache, pos, lengths),
+        h, n2 = add_mean_error_norm(h0, self.attn.decode_step(n1, cache, pos, lengths, position),
+                                    self.norm2.weight, self.norm2.eps, _narrow(h0))
+        return h, self.ffn(n2)
+
+    def tree_pending(self, x: torch.Tensor, r: Optional[torch.Tensor], cache, *tree):
+        """forward_pending for drafted tokens (AlgebraicAttention.forward_tree)."""
+        if r is None:
+            h0, n1 = x, self.norm1(x)
+        else:
+            h0, n1 = add_mean_error_norm(x, r, self.norm1.weight, self.norm1.eps, _narrow(x))
+        h, n2 = add_mean_error_norm(h0, self.attn.forward_tree(n1, cache, *tree),
                                     self.norm2.weight, self.norm2.eps, _narrow(h0))
         return h, self.ffn(n2)
 
@@ -299,21 +401,57 @@ class AlgebraicTransformerLM(nn.Module):
             x, r, self.norm.weight, self.norm.eps, _narrow(x))[1]
         return self.head(normed)
 
-    def decode_step(self, tokens: torch.Tensor, caches, pos: torch.Tensor,
-                    lengths: torch.Tensor) -> torch.Tensor:
-        """Logits [B, vocab] of one new token per row (tokens: [B, 1]) at the
-        device-side position ``pos`` (int64 [1]; ``lengths`` = pos + 1, int32
-        [B]) over filled ``caches``. Capturable in a HIP graph."""
+    def forward_tree(self, tokens: torch.Tensor, parents: torch.Tensor, caches, n: int,
+                     position: Optional[int] = None) -> torch.Tensor:
+        """Logits [B, N, vocab] of N <= 64 drafted tokens (tokens: [B, N]) over
+        caches with ``n`` filled rows, each token after the context and its
+        ancestors: ``parents`` (int32 [N] or [B, N]) names the token each one
+        follows, -1 the context. The tokens' keys and values go into the rows
+        behind; accept_drafted() keeps those of one branch. ``position``: the
+        position a token right after the context has, where the caches are
+        bounded (rows are positions otherwise). Bounded caches' weights do not grow:
+        a drafted token may yet be rejected."""
+        B, N = tokens.shape
+        lengths = torch.full((B,), n + N, dtype=torch.int32, device=tokens.device)
+        parents = parents.to(device=tokens.device, dtype=torch.int32).expand(B, N)
+        positions = None
+        if caches[0].keep is not None:
+            i = torch.arange(N, device=tokens.device)
+            up = (parents[:, :, None] == i).float() + torch.eye(N, device=tokens.device)
+            depth = (torch.linalg.matrix_power(up, 64) > 0).sum(-1) - 1  # ancestors above each token
+            positions = (depth + (n if position is None else position)).to(torch.int32)
         x = self.embed(tokens)
         r = None
         for block, cache in zip(self.blocks, caches):
-            x, r = block.decode_pending(x, r, cache, pos, lengths)
+            x, r = block.tree_pending(x, r, cache, parents, n, lengths, positions)
+        _, normed = add_mean_error_norm(x, r, self.norm.weight, self.norm.eps, _narrow(x))
+        return self.head(normed)
+
+    @staticmethod
+    def accept_drafted(caches, n: int, path: torch.Tensor):
+        """Keep, of the tokens that forward_tree put behind ``n`` rows, those of
+        ``path`` (int64 [B, m], from the context down): they become rows n ..
+        n + m - 1."""
+        for cache in caches:
+            cache.accept(n, path)
+
+    def decode_step(self, tokens: torch.Tensor, caches, pos: torch.Tensor,
+                    lengths: torch.Tensor, position: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Logits [B, vocab] of one new token per row (tokens: [B, 1]) at the
+        device-side position ``pos`` (int64 [1]; ``lengths`` = pos + 1, int32
+        [B]) over filled ``caches`` (bounded ones: row ``pos``, and ``position``
+        int32 [1]). Capturable in a HIP graph."""
+        x = self.embed(tokens)
+        r = None
+        for block, cache in zip(self.blocks, caches):
+            x, r = block.decode_pending(x, r, cache, pos, lengths, position)
         _, normed = add_mean_error_norm(x, r, self.norm.weight, self.norm.eps, _narrow(x))
         return self.head(normed)[:, -1, :]
 
-    def new_kv_caches(self, max_len: int) -> list:
-        """One KVCache per block, for up to ``max_len`` positions."""
-        return [KVCache(max_len) for _ in self.blocks]
+    def new_kv_caches(self, max_len: int, keep: Optional[int] = None, recent: int = 0) -> list:
+        """One KVCache per block, for up to ``max_len`` positions (with ``keep``:
+        bounded ones of ``max_len`` rows)."""
+        return [KVCache(max_len, keep, recent) for _ in self.blocks]
 
     @staticmethod
     def _sample(logits: torch.Tensor, temperature: float, top_k: Optional[int]) -> torch.Tensor:
@@ -328,7 +466,8 @@ class AlgebraicTransformerLM(nn.Module):
     @torch.no_grad()
     def generate(self, idx: torch.Tensor, max_new_tokens: int, temperature: float = 1.0,
                  top_k: Optional[int] = None, use_cache: bool = True,
-                 use_graph: bool = True) -> torch.Tensor:
+                 use_graph: bool = True, cache_keep: Optional[int] = None,
+                 cache_recent: Optional[int] = None) -> torch.Tensor:
         """Sample ``max_new_tokens`` tokens (reference algebraic_model.py:239-265).
 
         The reference re-runs the (cropped) prefix for every token. On CUDA
@@ -341,7 +480,17 @@ class AlgebraicTransformerLM(nn.Module):
         reference does. ``use_cache=False`` (or CPU tensors) always does.
         With ``use_graph`` the one-token decode step is captured once in a HIP
         graph and replayed per token (under autocast it is captured with the
-        autocast weight cache off, as graph capture requires)."""
+        autocast weight cache off, as graph capture requires).
+
+        ``cache_keep`` bounds the caches instead of the context (CUDA tensors): the
+        prompt's keys (of its last block_size tokens) and then every layer's and
+        head's keys are evicted down to those ``cache_keep`` that have received the
+        most attention weight, the ``cache_recent`` newest (default a quarter) always
+        among them, whenever an eighth as many more have been added. Generation
+        then goes on past block_size at a constant cost per token."""
+        if cache_keep is not None:
+            return self._generate_bounded(idx, max_new_tokens, temperature, top_k, use_graph,
+                                          cache_keep, cache_recent)
         T0 = idx.size(1)
         cached = use_cache and idx.is_cuda and max_new_tokens > 0 and T0 <= self.block_size
         caches = None
@@ -365,6 +514,68 @@ class AlgebraicTransformerLM(nn.Module):
         return idx
 
 
+    def _generate_bounded(self, idx, max_new_tokens, temperature, top_k, use_graph, keep, recent):
+        assert idx.is_cuda, "cache_keep needs CUDA tensors"
+        recent = keep // 4 if recent is None else recent
+        rows = keep + max(1, keep // 8)
+        caches = self.new_kv_caches(rows, keep, recent)
+        step = None
+        for i in range(max_new_tokens):
+            if i == 0:
+                ctx = idx[:, -self.block_size:]
+                logits = self.forward_cached(ctx, caches, 0)[:, -1, :]
+                n, position = min(ctx.size(1), keep), ctx.size(1)
+            else:
+                if n == rows:
+                    for cache in caches:
+                        cache.evict(n)
+                    n = keep
+                if step is None:
+                    step = _DecodeStep(self, caches, idx.size(0), idx.device, use_graph)
+                logits = step(idx[:, -1:], n, position)
+                n, position = n + 1, position + 1
+            nxt = self._sample(logits, temperature, top_k)
+            idx = torch.cat((idx, nxt), dim=1)
+        return idx
+
+    @torch.no_grad()
+    def generate_drafted(self, idx: torch.Tensor, max_new_tokens: int, draft) -> torch.Tensor:
+        """Greedy generation (the most likely token every time, as generate with
+        top_k = 1) of one sequence idx [1, T] (CUDA), several tokens per pass:
+        ``draft(idx)`` proposes what may follow as (tokens [N], parents [N]), N <
+        64, each token after the one its parent names, -1 directly after idx. One
+        forward_tree pass scores them all, and the branch that agrees with the
+        model is kept. The result does not depend on the drafts, up to float
+        rounding, only the number of passes does."""
+        assert idx.is_cuda and idx.size(0) == 1, "one sequence, on a CUDA device"
+        end = idx.size(1) + max_new_tokens
+        assert end <= self.block_size, "the context would be cropped"
+        if max_new_tokens <= 0:
+            return idx
+        caches = self.new_kv_caches(end + 64)
+        n = idx.size(1)
+        last = self.forward_cached(idx, caches, 0)[:, -1].argmax(-1, keepdim=True)
+        idx = torch.cat((idx, last), dim=1)
+        while idx.size(1) < end:
+            tokens, parents = (torch.as_tensor(t, device=idx.device).view(-1) for t in draft(idx))
+            tokens = torch.cat((last.view(-1), tokens.to(idx.dtype)))
+            parents = torch.cat((parents.new_full((1,), -1), parents + 1))  # the draft hangs on `last`
+            best = self.forward_tree(tokens[None], parents, caches, n).argmax(-1)[0].tolist()
+            toks, ups = tokens.tolist(), parents.tolist()
+            path = [0]
+            while True:
+                nxt = [j for j in range(path[-1] + 1, len(toks)) if ups[j] == path[-1] and toks[j] == best[path[-1]]]
+                if not nxt or idx.size(1) + len(path) >= end:
+                    break
+                path.append(nxt[0])
+            self.accept_drafted(caches, n, torch.tensor([path], device=idx.device))
+            n += len(path)
+            new = [toks[j] for j in path[1:]] + [best[path[-1]]]
+            idx = torch.cat((idx, torch.tensor([new], dtype=idx.dtype, device=idx.device)), dim=1)
+            last = idx[:, -1:]
+        return idx
+
+
 class _DecodeStep:
     """The model's one-token decode step over fixed caches, run eagerly or as a
     captured HIP graph: the token ids, position and lengths live in static
@@ -375,15 +586,18 @@ class _DecodeStep:
         self.tok = torch.zeros(batch, 1, dtype=torch.long, device=device)
         self.pos = torch.zeros(1, dtype=torch.long, device=device)
         self.lengths = torch.ones(batch, dtype=torch.int32, device=device)
+        self.position = torch.zeros(1, dtype=torch.int32, device=device)
         self.use_graph = use_graph
         self.graph = None
 
     def _run(self):
-        return self.model.decode_step(self.tok, self.caches, self.pos, self.lengths)
+        return self.model.decode_step(self.tok, self.caches, self.pos, self.lengths, self.position)
 
     def _capture(self):
         ac = torch.is_autocast_enabled()
         ac_dtype = torch.get_autocast_dtype("cuda") if ac else torch.float32
+        # (bounded caches: the warm-up's attention weights are not to count)
+        kept = [(c.weights, c.weights.clone()) for c in self.caches if c.weights is not None]
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
@@ -392,16 +606,19 @@ class _DecodeStep:
             with torch.autocast("cuda", dtype=ac_dtype, enabled=ac, cache_enabled=False):
                 self._run()
         torch.cuda.current_stream().wait_stream(side)
+        for weights, before in kept:
+            weights.copy_(before)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             with torch.autocast("cuda", dtype=ac_dtype, enabled=ac, cache_enabled=False):
                 self.logits = self._run()
         self.graph = graph
 
-    def __call__(self, tokens: torch.Tensor, pos: int) -> torch.Tensor:
+    def __call__(self, tokens: torch.Tensor, pos: int, position: int = 0) -> torch.Tensor:
         self.tok.copy_(tokens)
         self.pos.fill_(pos)
         self.lengths.fill_(pos + 1)
+        self.position.fill_(position)
         if not self.use_graph:
             return self._run()
         if self.graph is None:
