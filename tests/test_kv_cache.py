@@ -100,3 +100,50 @@ def test_evict_refusals():
     assert lib.kat_kv_evict(P, P, P, P, P, P, P, P, P, P, None, 0, 1, 2, 9, 64, 4, 0, 0, _lib.i64_array([64] * 20), 1,
                             None) == 1 and "lengths_out" in _msg()
     assert lib.kat_kv_evict_workspace_size(2, 3, 10) == 6 * 21 * 4
+
+
+# ------------------------------------------------- the oracle's own pins ----
+
+def test_oracle_rows_and_weights_are_those_of_the_attention():
+    import oracle as O
+    from oracle import cache as C
+    g = torch.Generator().manual_seed(0)
+    q, k, v = (torch.randn(1, 2, 23, 8, generator=g, dtype=torch.float64) for _ in range(3))
+    slopes = F.compute_alibi_slopes(2)
+    o, L = O.attention_fwd(q, k, v, slopes, 0.3)
+    for h in range(2):
+        cols = torch.zeros(23, dtype=torch.float64)
+        for i in (0, 7, 22):
+            dist = i - torch.arange(i + 1)
+            ro, rL, p, A, E = C.attention_rows(q[0, h, i], k[0, h, :i + 1], v[0, h, :i + 1], slopes[h], 0.3, dist)
+            assert float((ro - o[0, h, i]).abs().max()) <= 1e-12 and abs(float(rL - L[0, h, i])) <= 1e-12
+            assert 0 < E < 1e-3 and bool((A >= ro.abs() - 1e-12).all())
+            cols[:i + 1] += p
+        w = sum(C.key_weights(q[0, h, :i + 1], k[0, h, :i + 1], slopes[h], 0.3, L[0, h, :i + 1], None, 1)[0].new_zeros(23)
+                .index_add(0, torch.arange(i + 1), C.key_weights(q[0, h, :i + 1], k[0, h, :i + 1], slopes[h], 0.3,
+                                                                 L[0, h, :i + 1], None, 1)[0]) for i in (0, 7, 22))
+        assert float((w - cols).abs().max()) <= 1e-12
+        total, _ = C.key_weights(q[0, h], k[0, h], slopes[h], 0.3, L[0, h], None, None)
+        assert abs(float(total.sum()) - 23) <= 23 * 1e-4  # every query hands out L / (L + eps)
+
+
+def test_oracle_trees_and_evictions():
+    from oracle import cache as C
+    assert C.tree_lines([-1, 0, 0, 2, -1, 7, 4, -2, 7, 9]) == [[0], [0, 1], [0, 2], [0, 2, 3], [4], None, [4, 6],
+                                                               None, None, None]
+    pos = [0, 1, 2, 3, 4, 5]
+    assert C.evict_rows([3.0, 1.0, 3.0, 0.0, 2.0, 0.0], pos, 6, 3, 0) == [0, 2, 4]
+    assert C.evict_rows([3.0, 1.0, 3.0, 0.0, 2.0, 0.0], pos, 6, 3, 2) == [0, 4, 5]
+    assert C.evict_rows([3.0, 3.0, 3.0, 0.0], pos, 4, 2, 0) == [0, 1]           # ties: the lower row
+    assert C.evict_rows([3.0, float("nan"), 4.0, 0.0], pos, 4, 2, 0) == [1, 2]  # a NaN above every number
+    assert C.evict_rows([3.0, 1.0], pos, 2, 5, 1) == [0, 1]
+
+
+@pytest.mark.parametrize("B,H,T", [(1, 1, 1), (16, 16, 4096), (1, 8, 100000)])
+def test_workspaces_are_bounded(B, H, T):
+    # the partial sums of a call stay a small part of the cache it reads
+    lib = _lib.load()
+    cache = 2 * B * H * T * 128 * 2
+    assert lib.kat_attn_tree_workspace_size(B, H, 64, T, 128, 1) <= max(cache, 64 << 20)
+    assert lib.kat_attn_decode_accum_workspace_size(B, H, T, 128, 1) <= max(cache // 8, 8 << 20)
+    assert lib.kat_attn_key_weights_workspace_size(B, H, T, 128, 64, 1) <= max(cache // 8, 8 << 20)
