@@ -49,12 +49,12 @@ template <typename T, int W> constexpr int kw_units() { return W * (int)sizeof(T
 // query rows per LDS tile
 template <int U> constexpr int kw_rows() { return U == 512 ? 32 : 64; }
 
-// KS: 16-key subtiles per wave (their fragments take U / 8 registers each). QW:
-// waves that share their keys and split a tile's queries (1 or 4)
+// KS: 16-key subtiles per wave (their fragments take U / 8 registers each). QW > 1:
+// the block's QW waves share their keys and split a tile's queries (16 rows each)
 template <typename T, int W, bool KM, int KS, int QW>
-__global__ __launch_bounds__(64 * kKwWaves, (kw_units<T, W>() == 512 ? 1 : 2)) void attn_keyw_k(KeywArgs a) {
-  constexpr int ES = (int)sizeof(T), U = kw_units<T, W>(), KK = U / 32, QR = kw_rows<U>() * (QW == 4 && U == 512 ? 2 : 1);
-  constexpr int KWV = kKwWaves / QW;   // waves with keys of their own
+__global__ __launch_bounds__(64 * (QW > 1 ? QW : kKwWaves), (kw_units<T, W>() == 512 ? 1 : 2)) void attn_keyw_k(KeywArgs a) {
+  constexpr int ES = (int)sizeof(T), U = kw_units<T, W>(), KK = U / 32, NW = QW > 1 ? QW : kKwWaves, QR = QW > 1 ? 16 * QW : kw_rows<U>();
+  constexpr int KWV = NW / QW;   // waves with keys of their own
   constexpr int BK = 16 * KS * KWV;    // keys per block
   constexpr int WR = QR / QW;          // rows of a tile per wave
   constexpr bool kBiasC = ES == 2;     // the bias enters the product as its C operand
@@ -84,7 +84,7 @@ __global__ __launch_bounds__(64 * kKwWaves, (kw_units<T, W>() == 512 ? 1 : 2)) v
   const float scale = !kBiasC || fabsf(a.scale) >= 0x1p-60f ? a.scale : copysignf(0x1p-60f, a.scale);
   const int cols = a.D * ES / 16;
 
-  TileDma<U, kKwWaves, QR> dq;
+  TileDma<U, NW, QR> dq;
   dq.init(w, lane, (uint32_t)(sqb / 2), a.D * ES / 2);
   auto issue = [&](short* tile, int row) __attribute__((always_inline)) {
     const int64_t left = (int64_t)(T_ - 1 - row) * sqb + a.D * ES;  // bytes from this row to the last one's end
@@ -243,15 +243,18 @@ static int keyw_layout(int64_t D, int dtype) {
 //  - With fewer than three such blocks per CU the queries are split too. Up to 1024
 //    rows over the four waves of a block that share 16 keys, in one launch: bf16, D=64,
 //    chunks / waves: 12 heads, T=256 5.9 / 4.3; 48 heads, T=512 9.3 / 7.6; 24 heads,
-//    T=1000 12.3 / 10.9 (12 heads 9.6 / 9.9, and 16.6 / 18.4 at T=2048). Beyond, in
+//    T=1000 12.3 / 10.9 (12 heads 9.6 / 9.9, and 16.6 / 18.4 at T=2048); over eight
+//    waves while there are fewer than three such blocks per CU (four / eight waves: 12
+//    heads, T=512, D=128 7.2 / 6.3, T=1000, D=64 10.0 / 7.8; 24 heads, T=512, D=64 6.3 /
+//    6.4, in fp32 11.3 / 12.9; 96 heads, T=256 6.2 / 8.4). Beyond 1024 rows, in
 //    chunks over blocks, about four per CU, and a second launch: fp32, 12 heads,
 //    T=2048 53 us in two chunks, 44.8 in six.
 //  - Else one block takes all its queries, the longest first (64 heads, T=4096: 194 us
-//    whole, 207 in two chunks; 96 heads, T=512 8.9 whole, 11.7 split over waves).
+//    whole, 207 in two chunks; 96 heads, T=512 8.9 whole, 11.7 split over four waves).
 struct KeywPlan {
   int ks, qw, bk, qc, chunks;
 };
-static KeywPlan keyw_plan(int64_t B, int64_t H, int64_t T, int64_t lo, int dtype) {
+static KeywPlan keyw_plan(int64_t B, int64_t H, int64_t T, int64_t lo, int W, int dtype) {
   const int64_t cus = num_cus(), bh = B * H;
   KeywPlan p = {1, 1, 0, 0, 0};
   const double pairs = (double)bh * ((double)(T - lo) * lo + 0.5 * (T - lo) * (T - lo));
@@ -263,7 +266,7 @@ static KeywPlan keyw_plan(int64_t B, int64_t H, int64_t T, int64_t lo, int dtype
   if ((T + p.bk - 1) / p.bk * bh < 3 * cus) c = std::max<int64_t>(64, (rows * bh + 4 * cus - 1) / (4 * cus));
   c = (c + 63) / 64 * 64;  // whole tiles
   if (c < T - lo && p.ks == 1 && T <= 1024) {
-    p.qw = kKwWaves;
+    p.qw = (T + 15) / 16 * bh < 3 * cus && W * dtype_size(dtype) <= 512 ? 8 : 4;
     p.bk = 16;
     c = (T - lo + 63) / 64 * 64;
   }
@@ -273,17 +276,20 @@ static KeywPlan keyw_plan(int64_t B, int64_t H, int64_t T, int64_t lo, int dtype
 }
 
 template <typename T, int W, int KS, int QW> static int launch_keyw(const KeywArgs& a, hipStream_t st) {
-  constexpr int BK = 16 * KS * kKwWaves / QW;
+  constexpr int BK = 16 * KS * (QW > 1 ? 1 : kKwWaves);
   const dim3 grid((unsigned)((a.T + BK - 1) / BK * a.B * a.H), (unsigned)a.chunks);
-  if (a.mask) hipLaunchKernelGGL((attn_keyw_k<T, W, true, KS, QW>), grid, dim3(64 * kKwWaves), 0, st, a);
-  else hipLaunchKernelGGL((attn_keyw_k<T, W, false, KS, QW>), grid, dim3(64 * kKwWaves), 0, st, a);
+  if (a.mask) hipLaunchKernelGGL((attn_keyw_k<T, W, true, KS, QW>), grid, dim3(64 * (QW > 1 ? QW : kKwWaves)), 0, st, a);
+  else hipLaunchKernelGGL((attn_keyw_k<T, W, false, KS, QW>), grid, dim3(64 * (QW > 1 ? QW : kKwWaves)), 0, st, a);
   if (int rc = check_launch("kat_attn_key_weights")) return rc;
   if (!a.part) return KAT_OK;
   hipLaunchKernelGGL(attn_keyw_sum_k, dim3((unsigned)((a.T + 255) / 256), (unsigned)(a.B * a.H)), dim3(256), 0, st, a, BK);
   return check_launch("kat_attn_key_weights (sum)");
 }
 template <typename T, int W> static int keyw_mode(const KeywArgs& a, const KeywPlan& p, hipStream_t st) {
-  if (p.qw == kKwWaves) return launch_keyw<T, W, 1, kKwWaves>(a, st);
+  if constexpr (kw_units<T, W>() <= 256) {
+    if (p.qw == 8) return launch_keyw<T, W, 1, 8>(a, st);
+  }
+  if (p.qw == 4) return launch_keyw<T, W, 1, 4>(a, st);
   if constexpr (sizeof(T) == 2) {
     if (p.ks == 2) return launch_keyw<T, W, 2, 1>(a, st);
   }
@@ -307,7 +313,7 @@ extern "C" size_t kat_attn_key_weights_workspace_size(int64_t B, int64_t H, int6
                                                       int dtype) {
   const int W = keyw_layout(D, dtype);
   if (B <= 0 || H <= 0 || T <= 0 || last < 0 || !W) return 0;
-  const int chunks = keyw_plan(B, H, T, last == 0 ? 0 : std::max<int64_t>(0, T - last), dtype).chunks;
+  const int chunks = keyw_plan(B, H, T, last == 0 ? 0 : std::max<int64_t>(0, T - last), W, dtype).chunks;
   return chunks == 1 ? 0 : (size_t)chunks * B * H * T * sizeof(float);
 }
 
@@ -354,7 +360,7 @@ extern "C" int kat_attn_key_weights(const void* q, const void* k, const float* L
   a.so[1] = strides[10];
   a.scale = scale;
   a.eps = eps;
-  const KeywPlan p = keyw_plan(B, H, T, a.lo, dtype);
+  const KeywPlan p = keyw_plan(B, H, T, a.lo, W, dtype);
   a.qc = p.qc;
   a.chunks = p.chunks;
   const size_t need = kat_attn_key_weights_workspace_size(B, H, T, D, last, dtype);

@@ -284,13 +284,16 @@ template <int NT, int R, bool ONE> __global__ __launch_bounds__(NT) void kv_evic
     int nm = 0;
     each_kept([&](bool y, int) { nm += y; });
     int m0 = before(nm, tot[1]);
+    const int m1 = m0 + tot[1][wv];
     const int first = (int)blockIdx.x * a.share, last = min(first + a.share, m);
-    each_kept([&](bool y, int j) {
-      const uint64_t mm = __builtin_amdgcn_ballot_w64(y);
-      const int r = m0 + bits_below(mm) - first;
-      if (y && r >= 0 && r < last - first) list[r] = j;
-      m0 += __popcll(mm);
-    });
+    if (m0 < last && m1 > first) {  // else this wave's rows are other blocks'
+      each_kept([&](bool y, int j) {
+        const uint64_t mm = __builtin_amdgcn_ballot_w64(y);
+        const int r = m0 + bits_below(mm) - first;
+        if (y && r >= 0 && r < last - first) list[r] = j;
+        m0 += __popcll(mm);
+      });
+    }
     __syncthreads();
     if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0 && a.lo) a.lo[b] = m;
     move_rows<NT>(a, b, h, first, last, list, nullptr);
