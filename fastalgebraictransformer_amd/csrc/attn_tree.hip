@@ -25,8 +25,8 @@
 // tile:
 //   S^T[row][q] = K Q^T    A = K (LDS rows)             B = Q^T (registers)
 //   f of S^T               lane (g, li) holds rows 4 g + j, query li
-//   O^T[d][q] += V^T f^T   A = V^T (LDS, transposed reads)  B = f packed to the
-//                          dtype as the forward does, or fp32
+//   O^T[d][q] += V^T f^T   A = V^T (LDS, transposed reads)  B = f in two parts of
+//                          the dtype (Split), or fp32
 // A first version gave every wave whole rows for all queries, loaded straight
 // into registers: at 64 queries the accumulators and fragments (192 registers)
 // left no room for the rows in flight, and it spilled (578 us at B=8, H=16, N=64,
@@ -83,6 +83,25 @@ constexpr TreeShape tree_shape(int U, int QG) {
                                : TreeShape{32, 4, 4, U == 128 ? 2 : 1};
 }
 constexpr int tree_qg(int64_t N) { return N <= 16 ? 1 : N <= 32 ? 2 : 4; }
+
+// Two fp32 weights as packed pairs of T, the rounded values and what the rounding
+// left: the product with V then has the weights to 16 bits (bf16; 22 in fp16) and o
+// is rounded once, when it is stored. With the rounded weights alone, one rounding of
+// a weight near 1 moves a whole row of o by up to half a step of T (1.4 to 1.7 times
+// the error of o against 64 bits). B=8, H=16, T=8192, D=128, bf16, rounded / split: 64
+// tokens 95 / 103 us, 32 99 / 99, 16 94 / 94.
+template <typename T> struct Split {
+  uint32_t hi, lo;
+  __device__ __forceinline__ Split(float x, float y) {
+    hi = mfma::Mfma<T>::pack2(x, y);
+    if constexpr (__is_same(T, bf16)) {
+      lo = mfma::Mfma<T>::pack2(x - __builtin_bit_cast(float, hi << 16), y - __builtin_bit_cast(float, hi & 0xffff0000u));
+    } else {
+      const VecT<f16, 2> h = __builtin_bit_cast(VecT<f16, 2>, hi);
+      lo = mfma::Mfma<T>::pack2(x - (float)h.v[0], y - (float)h.v[1]);
+    }
+  }
+};
 
 template <typename T, int W, int QG> constexpr TreeShape tree_at() { return tree_shape(W * (int)sizeof(T) / 2, QG); }
 
@@ -187,6 +206,7 @@ void attn_tree_k(TreeArgs a) {
   int qpos = 0;
   if (qi < N && n > 0) qpos = POS ? pp[c + qi] : c + sdep[qi];
 
+  const float sj[4] = {0.f, slope, 2.f * slope, 3.f * slope};
   f32x4 oacc[DS];
   float lsum = 0.f;
 #pragma unroll
@@ -201,15 +221,26 @@ void attn_tree_k(TreeArgs a) {
     for (int kk = 0; kk < KK; ++kk) f = dot64<T>(lds16(kt + soff<U>(hr + li, 32 * kk + 8 * g)), qf[kk], f);
     i32x4 kpos;
     if constexpr (POS) kpos = *reinterpret_cast<const i32x4*>(pt + hr + 4 * g);
+    // (context rows that are positions: the lane's first one; the others lie j on)
+    const float bias0 = -slope * (float)(qpos - (k0 + hr + 4 * g));
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int row = k0 + hr + 4 * g + j;
-      const int tok = row - c;  // the drafted token in this row, if >= 0
-      int kp_ = row;
-      if constexpr (POS) kp_ = kpos[j];
-      else if constexpr (TAIL) kp_ = tok < 0 ? row : c + sdep[min(tok, kTreeMax - 1)];
-      const float s = fmaf(f[j], scale, -slope * (float)(qpos - kp_));
-      float x = sig2_pow4(s);
+      const int tok = k0 + hr + 4 * g + j - c;  // the drafted token in this row, if >= 0
+      float bias;
+      if constexpr (POS) bias = -slope * (float)(qpos - kpos[j]);
+      else if constexpr (TAIL) bias = -slope * (float)(qpos - (tok < 0 ? c + tok : c + sdep[min(tok, kTreeMax - 1)]));
+      else bias = j ? bias0 + sj[j] : bias0;
+      const float s = fmaf(f[j], scale, bias);
+      float x;
+      if constexpr (ES == 4) {
+        x = sig2_pow4(s);
+      } else {
+        // 1 + s r: two instructions less (B=8, H=16, N=64, T=8192, D=128 103 us, 110
+        // with sig2); its relative error, some 2^-22 (1 + |s|), grows only where f is
+        // small against the sums it enters
+        const float t = fmaf(s, __builtin_amdgcn_rcpf(fabsf(s) + 1.f), 1.f), t2 = t * t;
+        x = t2 * t2;
+      }
       if constexpr (TAIL) {
         const bool seen = tok < 0 ? anc != 0ull : tok < N && ((anc >> (tok & 63)) & 1ull);
         x = seen ? x : 0.f;
@@ -233,16 +264,23 @@ void attn_tree_k(TreeArgs a) {
                 *reinterpret_cast<const float*>(vt + soff<U>(hr + 16 * i + 4 * g + j, 32 * ds + 2 * li)),
                 i ? y[j] : x[j], oacc[ds], 0, 0, 0);
     } else if constexpr (RN == 32) {
-      const i16x8 pf = pack_frag(Mfma<T>::pack2(x[0], x[1]), Mfma<T>::pack2(x[2], x[3]), Mfma<T>::pack2(y[0], y[1]),
-                                 Mfma<T>::pack2(y[2], y[3]));
+      const Split<T> a0(x[0], x[1]), a1(x[2], x[3]), b0(y[0], y[1]), b1(y[2], y[3]);
+      const i16x8 ph = pack_frag(a0.hi, a1.hi, b0.hi, b1.hi), pl = pack_frag(a0.lo, a1.lo, b0.lo, b1.lo);
 #pragma unroll
-      for (int ds = 0; ds < DS; ++ds) oacc[ds] = Mfma<T>::mma(frag_tr<U>(vt, hr, 16 * ds, g, li), pf, oacc[ds]);
+      for (int ds = 0; ds < DS; ++ds) {
+        const i16x8 vf = frag_tr<U>(vt, hr, 16 * ds, g, li);
+        oacc[ds] = Mfma<T>::mma(vf, ph, oacc[ds]);
+        oacc[ds] = Mfma<T>::mma(vf, pl, oacc[ds]);
+      }
     } else {
-      const u32x2 p = u32x2{Mfma<T>::pack2(x[0], x[1]), Mfma<T>::pack2(x[2], x[3])};
+      const Split<T> a0(x[0], x[1]), a1(x[2], x[3]);
+      const i16x4 ph = __builtin_bit_cast(i16x4, (u32x2{a0.hi, a1.hi})), pl = __builtin_bit_cast(i16x4, (u32x2{a0.lo, a1.lo}));
 #pragma unroll
-      for (int ds = 0; ds < DS; ++ds)
-        oacc[ds] = mma_k16<T>(lds_tr(vt + soff<U>(hr + 4 * g + (li >> 2), 16 * ds + 4 * (li & 3))),
-                              __builtin_bit_cast(i16x4, p), oacc[ds]);
+      for (int ds = 0; ds < DS; ++ds) {
+        const i16x4 vf = lds_tr(vt + soff<U>(hr + 4 * g + (li >> 2), 16 * ds + 4 * (li & 3)));
+        oacc[ds] = mma_k16<T>(vf, ph, oacc[ds]);
+        oacc[ds] = mma_k16<T>(vf, pl, oacc[ds]);
+      }
     }
   };
   // the same for 16 rows without 0 x inf: rows with f = 0 add nothing

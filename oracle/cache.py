@@ -31,11 +31,11 @@ def _weights(q, k, slope, scale, dist, fused):
     return f, rel
 
 
-def attention_rows(q, k, v, slope, scale, dist, eps=EPS):
+def attention_rows(q, k, v, slope, scale, dist, eps=EPS, fused=False):
     """One query over the rows it sees: (o, L, p, A, E): p the attention
     weights, A = sum p |v|, E the largest relative error of an f."""
     q, k, v = q.double().cpu(), k.double().cpu(), v.double().cpu()
-    f, rel = _weights(q, k, float(slope), scale, dist.double().cpu(), False)
+    f, rel = _weights(q, k, float(slope), scale, dist.double().cpu(), fused)
     L = f.sum()
     p = f / (L + eps)
     e = float(rel.max()) if len(rel) else 0.0

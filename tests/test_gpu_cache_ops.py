@@ -5,10 +5,10 @@ Tolerances, derived before any run. u = finfo.eps / 2 of the tensors' type. An
 attention output o = sum p v is off by at most
     (2 E + r) A + u |o| + floor,   A = sum p |v|,
 E the relative error of an fp32 weight (the oracle's bound; once in the
-products and once in L), r = u for 16-bit types, whose weights enter the
-product of a tree in the tensors' type, and 0 for fp32; fp16 weights below its
-normal range (16 f < 2^-14) are off by 2^-25 absolutely, so floor = 2^-25 sum
-|v| / (16 (L + eps)). L is off by E L, a weight p by 2 E p + u32 p."""
+products and once in L), r = u^2 for 16-bit types, whose weights enter the
+product of a tree as a rounded value and the rounded rest, and 0 for fp32; fp16
+weights below its normal range (16 f < 2^-14) are off by 2^-25 absolutely, so
+floor = 2^-25 sum |v| / (16 (L + eps)). L is off by E L, a weight p by 2 E p + u32 p."""
 
 import math
 
@@ -45,7 +45,7 @@ def positions_like(B, H, T, seed):
 
 def check_out(got, ref, A, E, v, L, dtype, what, product_rounds):
     u = unit(dtype)
-    tol = (2 * E + (u if product_rounds and dtype != torch.float32 else 0.0)) * A + u * ref.abs() + 1e-30
+    tol = (2 * E + (u * u if product_rounds and dtype != torch.float32 else 0.0)) * A + u * ref.abs() + 1e-30
     if dtype == torch.float16 and product_rounds:
         tol = tol + 2.0 ** -25 * v.double().cpu().abs().sum(0) / (16 * (float(L) + 1e-6))
     if dtype == torch.float16:
@@ -87,7 +87,7 @@ def check_tree(o, L, q, k, v, slopes, scale, parents, lengths, positions, what="
                 rows = torch.tensor(list(range(c)) + [c + j for j in lines[i]])
                 at = torch.arange(c + len(lines[i])) if positions is None else positions[b, h].cpu()[rows]
                 ro, rL, _, A, E = C.attention_rows(qc[b, h, i], kc[b, h][rows], vc[b, h][rows], slopes[h],
-                                                   scale, at[-1] - at)
+                                                   scale, at[-1] - at, fused=q.dtype != torch.float32)
                 assert abs(float(L[b, h, i]) - float(rL)) <= E * float(rL), where
                 check_out(o[b, h, i], ro, A, E, vc[b, h][rows], rL, q.dtype, where, True)
 
