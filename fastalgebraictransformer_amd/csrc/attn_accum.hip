@@ -332,11 +332,15 @@ extern "C" int kat_attn_decode_accum(const void* q, const void* k, const void* v
   if (!q || !out || !slopes || !strides || !wp_strides || (T > 0 && (!k || !v || !weights)))
     return fail(KAT_EINVAL, "%s: null pointer", nm);
   const int esz = dtype_size(dtype);
-  for (int t = 0; t < 10; ++t)
-    if ((strides[t] * esz) % 16 != 0) return fail(KAT_EUNSUPPORTED, "%s: strides must keep rows 16-byte aligned", nm);
+  const int64_t size[10] = {B, H, B, H, T, B, H, T, B, H};
+  int64_t st10[10];
+  for (int t = 0; t < 10; ++t) {
+    st10[t] = dim_stride(strides[t], size[t]);
+    if ((st10[t] * esz) % 16 != 0) return fail(KAT_EUNSUPPORTED, "%s: strides must keep rows 16-byte aligned", nm);
+  }
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
     return fail(KAT_EUNSUPPORTED, "%s: tensors must be 16-byte aligned", nm);
-  if (T > 1 && (strides[4] < D || strides[7] < D)) return fail(KAT_EINVAL, "%s: cache row stride < D", nm);
+  if (T > 1 && (st10[4] < D || st10[7] < D)) return fail(KAT_EINVAL, "%s: cache row stride < D", nm);
   AccumArgs a = {};
   a.q = q;
   a.k = k;
@@ -352,14 +356,14 @@ extern "C" int kat_attn_decode_accum(const void* q, const void* k, const void* v
   a.T = (int)T;
   a.D = (int)D;
   for (int i = 0; i < 2; ++i) {
-    a.sq[i] = strides[i];
-    a.so[i] = strides[8 + i];
+    a.sq[i] = st10[i];
+    a.so[i] = st10[8 + i];
     a.stot[i] = wp_strides[i];
     a.spos[i] = wp_strides[2 + i];
   }
   for (int i = 0; i < 3; ++i) {
-    a.sk[i] = strides[2 + i];
-    a.sv[i] = strides[5 + i];
+    a.sk[i] = st10[2 + i];
+    a.sv[i] = st10[5 + i];
   }
   a.scale = scale;
   a.eps = eps;

@@ -331,12 +331,16 @@ extern "C" int kat_attn_key_weights(const void* q, const void* k, const float* L
   if (B * H * T == 0) return KAT_OK;
   if (!q || !k || !L || !weights || !slopes || !strides) return fail(KAT_EINVAL, "%s: null pointer", nm);
   const int esz = dtype_size(dtype);
-  for (int t = 0; t < 6; ++t)
-    if ((strides[t] * esz) % 16 != 0) return fail(KAT_EUNSUPPORTED, "%s: strides must keep rows 16-byte aligned", nm);
+  int64_t st6[6];
+  for (int t = 0; t < 6; ++t) {
+    const int64_t size[3] = {B, H, T};
+    st6[t] = dim_stride(strides[t], size[t % 3]);
+    if ((st6[t] * esz) % 16 != 0) return fail(KAT_EUNSUPPORTED, "%s: strides must keep rows 16-byte aligned", nm);
+  }
   if (!aligned16(q) || !aligned16(k)) return fail(KAT_EUNSUPPORTED, "%s: tensors must be 16-byte aligned", nm);
-  if (T > 1 && (strides[2] < D || strides[5] < D)) return fail(KAT_EINVAL, "%s: row stride < D", nm);
+  if (T > 1 && (st6[2] < D || st6[5] < D)) return fail(KAT_EINVAL, "%s: row stride < D", nm);
   // a tile's rows are addressed by 31-bit byte offsets
-  if (T > 1 && strides[2] * esz * 64 > 0x7fffffff) return fail(KAT_EUNSUPPORTED, "%s: q row stride too large", nm);
+  if (st6[2] > 0x7fffffff / (64 * esz)) return fail(KAT_EUNSUPPORTED, "%s: q row stride too large", nm);
   KeywArgs a = {};
   a.q = q;
   a.k = k;
@@ -351,11 +355,11 @@ extern "C" int kat_attn_key_weights(const void* q, const void* k, const float* L
   a.D = (int)D;
   a.lo = last == 0 ? 0 : (int)std::max<int64_t>(0, T - last);
   for (int i = 0; i < 3; ++i) {
-    a.sq[i] = strides[i];
-    a.sk[i] = strides[3 + i];
+    a.sq[i] = st6[i];
+    a.sk[i] = st6[3 + i];
     a.sl[i] = strides[6 + i];
   }
-  if (T == 1) a.sq[2] = D;  // one row: its stride may be anything
+  if (T == 1) a.sq[2] = D;
   a.so[0] = strides[9];
   a.so[1] = strides[10];
   a.scale = scale;

@@ -501,13 +501,17 @@ extern "C" int kat_attn_tree(const void* q, const void* k, const void* v, void* 
   if (!q || !out || !slopes || !parents || !strides || (positions && !pos_strides) || (T > 0 && (!k || !v)))
     return fail(KAT_EINVAL, "%s: null pointer", nm);
   const int esz = dtype_size(dtype);
-  for (int t = 0; t < 12; ++t)
-    if ((strides[t] * esz) % 16 != 0) return fail(KAT_EUNSUPPORTED, "%s: strides must keep rows 16-byte aligned", nm);
+  int64_t st12[12];
+  for (int t = 0; t < 12; ++t) {
+    const int64_t size[3] = {B, H, t < 3 || t >= 9 ? N : T};
+    st12[t] = dim_stride(strides[t], size[t % 3]);
+    if ((st12[t] * esz) % 16 != 0) return fail(KAT_EUNSUPPORTED, "%s: strides must keep rows 16-byte aligned", nm);
+  }
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
     return fail(KAT_EUNSUPPORTED, "%s: tensors must be 16-byte aligned", nm);
-  if (T > 1 && (strides[5] < D || strides[8] < D)) return fail(KAT_EINVAL, "%s: cache row stride < D", nm);
+  if (T > 1 && (st12[5] < D || st12[8] < D)) return fail(KAT_EINVAL, "%s: cache row stride < D", nm);
   // a tile's rows are addressed by 31-bit byte offsets
-  if (T > 1 && std::max(strides[5], strides[8]) > 0x7fffffff / (64 * esz))
+  if (T > 1 && std::max(st12[5], st12[8]) > 0x7fffffff / (64 * esz))
     return fail(KAT_EUNSUPPORTED, "%s: cache row stride too large", nm);
   TreeArgs a = {};
   a.q = q;
@@ -525,12 +529,12 @@ extern "C" int kat_attn_tree(const void* q, const void* k, const void* v, void* 
   a.T = (int)T;
   a.D = (int)D;
   for (int i = 0; i < 3; ++i) {
-    a.sq[i] = strides[i];
-    a.sk[i] = strides[3 + i];
-    a.sv[i] = strides[6 + i];
-    a.so[i] = strides[9 + i];
+    a.sq[i] = st12[i];
+    a.sk[i] = st12[3 + i];
+    a.sv[i] = st12[6 + i];
+    a.so[i] = st12[9 + i];
   }
-  if (T == 1) a.sk[2] = a.sv[2] = D;  // one row: its stride may be anything
+  if (T <= 1) a.sk[2] = a.sv[2] = D;
   a.spar = parents_stride_b;
   if (positions) {
     a.spos[0] = pos_strides[0];

@@ -21,6 +21,9 @@ inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// the stride of a dim: that of a dim of one element says nothing
+inline int64_t dim_stride(int64_t stride, int64_t size) { return size > 1 ? stride : 0; }
+
 inline int dtype_size(int dtype) {
   switch (dtype) {
     case KAT_F32: return 4;

@@ -375,8 +375,12 @@ extern "C" int kat_kv_evict(const void* k, const void* v, const float* weights, 
     return fail(KAT_EINVAL, "%s: null pointer", nm);
   if (in_place && (k != k_out || v != v_out || weights != weights_out || positions != positions_out))
     return fail(KAT_EINVAL, "%s: in place, but the outputs are other tensors", nm);
-  for (int t = 0; t < 12; ++t)
-    if ((strides[t] * esz) % 16 != 0) return fail(KAT_EUNSUPPORTED, "%s: strides must keep rows 16-byte aligned", nm);
+  int64_t st12[12];
+  for (int t = 0; t < 12; ++t) {
+    const int64_t size[3] = {B, H, t < 6 ? T : std::min(keep, T)};
+    st12[t] = dim_stride(strides[t], size[t % 3]);
+    if ((st12[t] * esz) % 16 != 0) return fail(KAT_EUNSUPPORTED, "%s: strides must keep rows 16-byte aligned", nm);
+  }
   if (!aligned16(k) || !aligned16(v) || !aligned16(k_out) || !aligned16(v_out))
     return fail(KAT_EUNSUPPORTED, "%s: tensors must be 16-byte aligned", nm);
   if (!in_place && lengths_out && lengths_out == lengths)
@@ -402,10 +406,10 @@ extern "C" int kat_kv_evict(const void* k, const void* v, const float* weights, 
   a.recent = (int)recent;
   a.pieces = (int)(D * esz / 16);
   for (int i = 0; i < 3; ++i) {
-    a.sk[i] = strides[i] * esz;
-    a.sv[i] = strides[3 + i] * esz;
-    a.sko[i] = strides[6 + i] * esz;
-    a.svo[i] = strides[9 + i] * esz;
+    a.sk[i] = st12[i] * esz;
+    a.sv[i] = st12[3 + i] * esz;
+    a.sko[i] = st12[6 + i] * esz;
+    a.svo[i] = st12[9 + i] * esz;
   }
   for (int i = 0; i < 2; ++i) {
     a.sw[i] = strides[12 + i];

@@ -143,6 +143,32 @@ def test_arguments_are_converted(gpu):
     assert same(res, again)
 
 
+def test_dims_of_one_element_have_no_stride(gpu):
+    # views whose strides of single-element dims are odd numbers
+    k, v = rand((1, 1, 40, 64), torch.bfloat16, 1), rand((1, 1, 40, 64), torch.bfloat16, 2)
+    q = rand((1, 1, 1, 64), torch.bfloat16, 3)
+    odd = lambda t, *s: t.as_strided(t.shape, s)
+    s = torch.tensor([0.1], device=dev)
+    root = torch.full((1,), -1, dtype=torch.int32, device=dev)
+    ko, vo, qo = odd(k, 3, 5, 64, 1), odd(v, 1, 7, 64, 1), odd(q, 3, 1, 5, 1)
+    want = F.rational_attention_tree(q, k, v, s, 0.2, root)
+    assert same(want, F.rational_attention_tree(qo, ko, vo, s, 0.2, root))
+    t1, t2 = torch.zeros(1, 1, 40, device=dev), torch.zeros(1, 1, 40, device=dev)
+    want = F.rational_attention_decode_accumulate(q[:, :, 0], k, v, s, 0.2, t1)
+    got = F.rational_attention_decode_accumulate(odd(q[:, :, 0], 3, 9, 1), ko, vo, s, 0.2, odd(t2, 1, 1, 1))
+    assert same(want, got) and torch.equal(t1, t2)
+    L = torch.rand(1, 1, 40, device=dev) + 1
+    assert torch.equal(F.rational_attention_key_weights(k, v, s, 0.2, L),
+                       F.rational_attention_key_weights(ko, vo, s, 0.2, odd(L, 3, 1, 1)))
+    one = (odd(q, 3, 1, 5, 1), odd(q.clone(), 7, 3, 1, 1), odd(torch.ones(1, 1, 1, device=dev), 0, 0, 0),
+           torch.zeros(1, 1, 1, dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev))
+    F.kv_cache_evict(ko, vo, t1, torch.arange(40, dtype=torch.int32, device=dev).view(1, 1, 40), None, 1, out=one)
+    j = int(t1[0, 0].argmax())
+    torch.cuda.synchronize()
+    assert torch.equal(one[0][0, 0, 0], k[0, 0, j]) and torch.equal(one[1][0, 0, 0], v[0, 0, j])
+    assert int(one[3]) == j and int(one[4]) == 1
+
+
 def test_empty_calls(gpu):
     s = F.compute_alibi_slopes(2).to(dev)
     kv = torch.zeros(3, 2, 0, 64, dtype=torch.bfloat16, device=dev)
