@@ -21,7 +21,7 @@
 //
 // A block streams its rows through LDS in tiles of 64 (LDS-DMA, a ring of
 // NS stages, non-temporal: each row is used once), so rows in flight hold no
-// registers. Its waves form QG query groups of 16 queries and KG row groups of a
+// registers. Its waves form QG query groups of 16 QT queries and KG row groups of a
 // tile:
 //   S^T[row][q] = K Q^T    A = K (LDS rows)             B = Q^T (registers)
 //   f of S^T               lane (g, li) holds rows 4 g + j, query li
@@ -64,25 +64,29 @@ struct TreeArgs {
 };
 
 constexpr int kTreeMax = 64;  // tokens: one ancestor mask is one 64-bit word
-// How a block is laid out, by a row's 16-bit units U and the query groups QG: rows
-// of a tile, waves, stages of the ring (a stage is 4 U bytes per row, of the CU's 160
-// KB of LDS) and blocks per CU. Eight waves run on a CU, in one block where the
-// registers allow it: it then streams one ring four stages deep, and there are half
-// the partial sums (B=8, H=16, N=64, T=8192, D=128: 90 us, against 103 with two
-// blocks of four waves and rings of two stages). At U = 256 eight waves of 64 queries
-// would spill; there, and for 32 queries at U = 128, four waves take tiles of 32 rows (B=4,
-// H=16, N=64, T=2048, D=256 41 us, with 64 43; B=3, H=16, N=25, T=1999, D=96 16.8, with
-// eight waves 19.1). A wave has 16 rows of a tile at least.
+// How a block is laid out, by a row's 16-bit units U and the number NQ of 16-query
+// subtiles (1, 2 or 4): rows of a tile, waves, stages of the ring (a stage is 4 U
+// bytes per row, of the CU's 160 KB of LDS), blocks per CU, and subtiles per wave.
+//  - Eight waves run on a CU, in one block where the registers allow it: it streams one
+//    ring four stages deep and leaves half the partial sums. B=8, H=16, N=64, T=8192,
+//    D=128, bf16 (weights rounded once): one block of eight 90 us, two of four waves
+//    with rings of two stages 103. At U = 256 eight waves of 64 queries would spill, and
+//    with 32 queries at U = 128 they leave each wave few rows: four waves there, on
+//    tiles of 32 rows. B=4, H=16, N=64, T=2048, D=256 tiles of 32 / 64 rows 41 / 43; B=3,
+//    H=16, N=25, T=1999, D=96 four / eight waves 16.8 / 19.1. A wave has 16 rows of a
+//    tile at least.
+//  - With 64 queries two subtiles per wave, which share its reads of K and V (one / two:
+//    B=16, H=12, T=4096, D=64 63.5 / 61.2, B=8, H=16, T=8192, D=128 107 / 105).
 struct TreeShape {
-  int rows, waves, stages, blocks;
+  int rows, waves, stages, blocks, qt;
 };
-constexpr TreeShape tree_shape(int U, int QG) {
-  return U <= 64 ? TreeShape{64, QG == 1 ? 4 : 8, 4, QG == 1 ? 2 : 1}
-         : QG == 1 ? TreeShape{64, 4, 2, U == 128 ? 2 : 1}
-         : U == 128 && QG == 4 ? TreeShape{64, 8, 4, 1}
-                               : TreeShape{32, 4, 4, U == 128 ? 2 : 1};
+constexpr TreeShape tree_shape(int U, int NQ) {
+  return U <= 64 ? TreeShape{64, NQ == 1 ? 4 : 8, 4, NQ == 1 ? 2 : 1, NQ == 4 ? 2 : 1}
+         : NQ == 1 ? TreeShape{64, 4, 2, U == 128 ? 2 : 1, 1}
+         : U == 128 && NQ == 4 ? TreeShape{64, 8, 4, 1, 2}
+                               : TreeShape{32, 4, 4, U == 128 ? 2 : 1, 1};
 }
-constexpr int tree_qg(int64_t N) { return N <= 16 ? 1 : N <= 32 ? 2 : 4; }
+constexpr int tree_nq(int64_t N) { return N <= 16 ? 1 : N <= 32 ? 2 : 4; }
 
 // Two fp32 weights as packed pairs of T, the rounded values and what the rounding
 // left: the product with V then has the weights to 16 bits (bf16; 22 in fp16) and o
@@ -103,26 +107,27 @@ template <typename T> struct Split {
   }
 };
 
-template <typename T, int W, int QG> constexpr TreeShape tree_at() { return tree_shape(W * (int)sizeof(T) / 2, QG); }
+template <typename T, int W, int NQ> constexpr TreeShape tree_at() { return tree_shape(W * (int)sizeof(T) / 2, NQ); }
 
-template <typename T, int W, int QG, bool POS>
-__global__ __launch_bounds__((64 * tree_at<T, W, QG>().waves), (tree_at<T, W, QG>().waves * tree_at<T, W, QG>().blocks / 4))
+template <typename T, int W, int NQ, bool POS>
+__global__ __launch_bounds__((64 * tree_at<T, W, NQ>().waves), (tree_at<T, W, NQ>().waves * tree_at<T, W, NQ>().blocks / 4))
 void attn_tree_k(TreeArgs a) {
   constexpr int ES = (int)sizeof(T);
   constexpr int U = W * ES / 2;          // a row in 16-bit units, the unit of the tile helpers
   constexpr int KK = U / 32;             // 64-byte column blocks
   constexpr int DS = W / 16;             // 16-wide d subtiles
-  constexpr TreeShape S = tree_at<T, W, QG>();
-  constexpr int NW = S.waves, TR = S.rows, NS = S.stages;
+  constexpr TreeShape S = tree_at<T, W, NQ>();
+  constexpr int NW = S.waves, TR = S.rows, NS = S.stages, QT = S.qt;
+  constexpr int QG = NQ / QT;            // query groups
   constexpr int KG = NW / QG;            // row groups of a tile
   constexpr int TK = TR / KG;            // rows of a wave's group
   typedef TileDma<U, NW, TR> Dma;
   constexpr int OPS = 2 * Dma::SEGS + (POS ? 1 : 0);  // a wave's DMA operations per tile
   constexpr int RING = NS * 2 * TR * U;
-  static_assert(TK >= 16 && RING * 2 >= NW * DS * 1024, "the ring holds the waves' sums");
+  static_assert(TK >= 16 && RING * 2 >= NW * DS * QT * 1024, "the ring holds the waves' sums");
   __shared__ __align__(16) short ring[RING];
   __shared__ int spos[POS ? NS : 1][NW][64];  // (a DMA writes 64 words)
-  __shared__ float sl[NW][16];
+  __shared__ float sl[NW][16 * QT];
   __shared__ uint64_t sanc[kTreeMax];  // ancestors of token i, itself included; 0 if absent
   __shared__ int sdep[kTreeMax];       // depth of token i below the context
 
@@ -135,16 +140,18 @@ void attn_tree_k(TreeArgs a) {
   const float slope = a.slopes[h], scale = a.scale;
   // what does not wait for the length: the queries and the parents
   const int cols = a.D * ES / 16;  // 16-byte pieces of a row that hold columns
-  const int qi = 16 * qg + li;     // the lane's token
-  i16x8 qf[KK];
+  const int qi = 16 * QT * qg + li;  // the lane's token of the first subtile; + 16 of the next
+  i16x8 qf[QT][KK];
 #pragma unroll
-  for (int kk = 0; kk < KK; ++kk) {
-    const int p = 4 * kk + g;
-    qf[kk] = i16x8{0, 0, 0, 0, 0, 0, 0, 0};
-    if (qi < N && p < cols)
-      qf[kk] = *reinterpret_cast<const i16x8*>((const char*)((const T*)a.q + b * a.sq[0] + h * a.sq[1] + qi * a.sq[2]) +
-                                               16 * p);
-  }
+  for (int qs = 0; qs < QT; ++qs)
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      const int p = 4 * kk + g, i = qi + 16 * qs;
+      qf[qs][kk] = i16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (i < N && p < cols)
+        qf[qs][kk] = *reinterpret_cast<const i16x8*>(
+            (const char*)((const T*)a.q + b * a.sq[0] + h * a.sq[1] + i * a.sq[2]) + 16 * p);
+    }
   const int parent = w == 0 && lane < N ? a.parents[b * a.spar + lane] : -2;
   int n = a.lengths ? a.lengths[b] : a.T;
   n = min(n, a.T);
@@ -202,104 +209,139 @@ void attn_tree_k(TreeArgs a) {
   }
 
   __syncthreads();  // masks and depths
-  const uint64_t anc = qi < N ? sanc[qi] : 0ull;
-  int qpos = 0;
-  if (qi < N && n > 0) qpos = POS ? pp[c + qi] : c + sdep[qi];
+  uint64_t anc[QT];
+  int qpos[QT];
+#pragma unroll
+  for (int qs = 0; qs < QT; ++qs) {
+    const int i = qi + 16 * qs;
+    anc[qs] = i < N ? sanc[i] : 0ull;
+    qpos[qs] = 0;
+    if (i < N && n > 0) qpos[qs] = POS ? pp[c + i] : c + sdep[i];
+  }
 
   const float sj[4] = {0.f, slope, 2.f * slope, 3.f * slope};
-  f32x4 oacc[DS];
-  float lsum = 0.f;
+  f32x4 oacc[DS][QT];
+  float lsum[QT];
 #pragma unroll
-  for (int ds = 0; ds < DS; ++ds) oacc[ds] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int qs = 0; qs < QT; ++qs) {
+    lsum[qs] = 0.f;
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) oacc[ds][qs] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
 
   // 16 rows at tile row hr (row k0 + hr of the cache) against the wave's
   // queries: f of S^T. TAIL: the tile reaches the tokens' rows or the end
-  auto scores = [&](auto tail_tag, int k0, int hr, const short* kt, const int* pt) __attribute__((always_inline)) {
+  auto scores = [&](auto tail_tag, int k0, int hr, const short* kt, const int* pt, f32x4 (&f)[QT]) __attribute__((always_inline)) {
     constexpr bool TAIL = decltype(tail_tag)::value;
-    f32x4 f = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) f = dot64<T>(lds16(kt + soff<U>(hr + li, 32 * kk + 8 * g)), qf[kk], f);
+    for (int qs = 0; qs < QT; ++qs) f[qs] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      const i16x8 kf = lds16(kt + soff<U>(hr + li, 32 * kk + 8 * g));
+#pragma unroll
+      for (int qs = 0; qs < QT; ++qs) f[qs] = dot64<T>(kf, qf[qs][kk], f[qs]);
+    }
     i32x4 kpos;
     if constexpr (POS) kpos = *reinterpret_cast<const i32x4*>(pt + hr + 4 * g);
-    // (context rows that are positions: the lane's first one; the others lie j on)
-    const float bias0 = -slope * (float)(qpos - (k0 + hr + 4 * g));
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int tok = k0 + hr + 4 * g + j - c;  // the drafted token in this row, if >= 0
-      float bias;
-      if constexpr (POS) bias = -slope * (float)(qpos - kpos[j]);
-      else if constexpr (TAIL) bias = -slope * (float)(qpos - (tok < 0 ? c + tok : c + sdep[min(tok, kTreeMax - 1)]));
-      else bias = j ? bias0 + sj[j] : bias0;
-      const float s = fmaf(f[j], scale, bias);
-      float x;
-      if constexpr (ES == 4) {
-        x = sig2_pow4(s);
-      } else {
-        // 1 + s r: two instructions less (B=8, H=16, N=64, T=8192, D=128 103 us, 110
-        // with sig2); its relative error, some 2^-22 (1 + |s|), grows only where f is
-        // small against the sums it enters
-        const float t = fmaf(s, __builtin_amdgcn_rcpf(fabsf(s) + 1.f), 1.f), t2 = t * t;
-        x = t2 * t2;
+    for (int qs = 0; qs < QT; ++qs) {
+      // (context rows that are positions: the lane's first one; the others lie j on)
+      const float bias0 = -slope * (float)(qpos[qs] - (k0 + hr + 4 * g));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int tok = k0 + hr + 4 * g + j - c;  // the drafted token in this row, if >= 0
+        float bias;
+        if constexpr (POS) bias = -slope * (float)(qpos[qs] - kpos[j]);
+        else if constexpr (TAIL) bias = -slope * (float)(qpos[qs] - (tok < 0 ? c + tok : c + sdep[min(tok, kTreeMax - 1)]));
+        else bias = j ? bias0 + sj[j] : bias0;
+        const float s = fmaf(f[qs][j], scale, bias);
+        float x;
+        if constexpr (ES == 4) {
+          x = sig2_pow4(s);
+        } else {
+          // 1 + s r: two instructions less (B=8, H=16, N=64, T=8192, D=128 103 us, 110
+          // with sig2); its relative error, some 2^-22 (1 + |s|), grows only where f is
+          // small against the sums it enters
+          const float t = fmaf(s, __builtin_amdgcn_rcpf(fabsf(s) + 1.f), 1.f), t2 = t * t;
+          x = t2 * t2;
+        }
+        if constexpr (TAIL) {
+          const bool seen = tok < 0 ? anc[qs] != 0ull : tok < N && ((anc[qs] >> (tok & 63)) & 1ull);
+          x = seen ? x : 0.f;
+        }
+        f[qs][j] = x;
       }
-      if constexpr (TAIL) {
-        const bool seen = tok < 0 ? anc != 0ull : tok < N && ((anc >> (tok & 63)) & 1ull);
-        x = seen ? x : 0.f;
-      }
-      f[j] = x;
+      lsum[qs] += (f[qs][0] + f[qs][1]) + (f[qs][2] + f[qs][3]);
     }
-    lsum += (f[0] + f[1]) + (f[2] + f[3]);
-    return f;
   };
-  // O^T += V^T f^T over RN rows (16 or 32) at tile row hr
-  auto product = [&](auto rn_tag, int hr, const f32x4& x, const f32x4& y, const short* vt) __attribute__((always_inline)) {
-    constexpr int RN = decltype(rn_tag)::value;
+  // O^T += V^T f^T over the 32 rows at tile row hr (x: the first 16, y), or over 16
+  auto product32 = [&](int hr, const f32x4 (&x)[QT], const f32x4 (&y)[QT], const short* vt) __attribute__((always_inline)) {
+    if constexpr (ES == 2) {
+      i16x8 ph[QT], pl[QT];
+#pragma unroll
+      for (int qs = 0; qs < QT; ++qs) {
+        const Split<T> a0(x[qs][0], x[qs][1]), a1(x[qs][2], x[qs][3]), b0(y[qs][0], y[qs][1]), b1(y[qs][2], y[qs][3]);
+        ph[qs] = pack_frag(a0.hi, a1.hi, b0.hi, b1.hi);
+        pl[qs] = pack_frag(a0.lo, a1.lo, b0.lo, b1.lo);
+      }
+#pragma unroll
+      for (int ds = 0; ds < DS; ++ds) {
+        const i16x8 vf = frag_tr<U>(vt, hr, 16 * ds, g, li);
+#pragma unroll
+        for (int qs = 0; qs < QT; ++qs) oacc[ds][qs] = Mfma<T>::mma(vf, ph[qs], oacc[ds][qs]);
+#pragma unroll
+        for (int qs = 0; qs < QT; ++qs) oacc[ds][qs] = Mfma<T>::mma(vf, pl[qs], oacc[ds][qs]);
+      }
+    }
+  };
+  auto product16 = [&](int hr, const f32x4 (&x)[QT], const short* vt) __attribute__((always_inline)) {
     if constexpr (ES == 4) {
 #pragma unroll
       for (int ds = 0; ds < DS; ++ds)
 #pragma unroll
-        for (int i = 0; i < RN / 16; ++i)
+        for (int j = 0; j < 4; ++j) {
+          const float vf = *reinterpret_cast<const float*>(vt + soff<U>(hr + 4 * g + j, 32 * ds + 2 * li));
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            oacc[ds] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                *reinterpret_cast<const float*>(vt + soff<U>(hr + 16 * i + 4 * g + j, 32 * ds + 2 * li)),
-                i ? y[j] : x[j], oacc[ds], 0, 0, 0);
-    } else if constexpr (RN == 32) {
-      const Split<T> a0(x[0], x[1]), a1(x[2], x[3]), b0(y[0], y[1]), b1(y[2], y[3]);
-      const i16x8 ph = pack_frag(a0.hi, a1.hi, b0.hi, b1.hi), pl = pack_frag(a0.lo, a1.lo, b0.lo, b1.lo);
-#pragma unroll
-      for (int ds = 0; ds < DS; ++ds) {
-        const i16x8 vf = frag_tr<U>(vt, hr, 16 * ds, g, li);
-        oacc[ds] = Mfma<T>::mma(vf, ph, oacc[ds]);
-        oacc[ds] = Mfma<T>::mma(vf, pl, oacc[ds]);
-      }
+          for (int qs = 0; qs < QT; ++qs)
+            oacc[ds][qs] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, x[qs][j], oacc[ds][qs], 0, 0, 0);
+        }
     } else {
-      const Split<T> a0(x[0], x[1]), a1(x[2], x[3]);
-      const i16x4 ph = __builtin_bit_cast(i16x4, (u32x2{a0.hi, a1.hi})), pl = __builtin_bit_cast(i16x4, (u32x2{a0.lo, a1.lo}));
+      // one product takes both parts of the weights: 32 k-indices, the rows twice
+      i16x8 p[QT];
+#pragma unroll
+      for (int qs = 0; qs < QT; ++qs) {
+        const Split<T> a0(x[qs][0], x[qs][1]), a1(x[qs][2], x[qs][3]);
+        p[qs] = pack_frag(a0.hi, a1.hi, a0.lo, a1.lo);
+      }
 #pragma unroll
       for (int ds = 0; ds < DS; ++ds) {
-        const i16x4 vf = lds_tr(vt + soff<U>(hr + 4 * g + (li >> 2), 16 * ds + 4 * (li & 3)));
-        oacc[ds] = mma_k16<T>(vf, ph, oacc[ds]);
-        oacc[ds] = mma_k16<T>(vf, pl, oacc[ds]);
+        const i16x4 v = lds_tr(vt + soff<U>(hr + 4 * g + (li >> 2), 16 * ds + 4 * (li & 3)));
+        const i16x8 vf = i16x8{v[0], v[1], v[2], v[3], v[0], v[1], v[2], v[3]};
+#pragma unroll
+        for (int qs = 0; qs < QT; ++qs) oacc[ds][qs] = Mfma<T>::mma(vf, p[qs], oacc[ds][qs]);
       }
     }
   };
-  // the same for 16 rows without 0 x inf: rows with f = 0 add nothing
-  auto product_checked = [&](int hr, const f32x4& x, const short* vt) __attribute__((always_inline)) {
+  // the same without 0 x inf: rows with f = 0 add nothing
+  auto product_checked = [&](int hr, const f32x4 (&x)[QT], const short* vt) __attribute__((always_inline)) {
     for (int r = 0; r < 16; ++r) {
       const int src = (r >> 2) * 16 + li;  // the lane that holds this row's f of query li
-      float y = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float z = __shfl(x[j], src, 64);
-        if ((r & 3) == j) y = z;
-      }
-#pragma unroll
-      for (int ds = 0; ds < DS; ++ds)
+      for (int qs = 0; qs < QT; ++qs) {
+        float y = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const T z = *reinterpret_cast<const T*>(vt + soff<U>(hr + r, (16 * ds + 4 * g + j) * ES / 2));
-          if (y != 0.f) oacc[ds][j] = fmaf(y, (float)z, oacc[ds][j]);
+          const float z = __shfl(x[qs][j], src, 64);
+          if ((r & 3) == j) y = z;
         }
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const T z = *reinterpret_cast<const T*>(vt + soff<U>(hr + r, (16 * ds + 4 * g + j) * ES / 2));
+            if (y != 0.f) oacc[ds][qs][j] = fmaf(y, (float)z, oacc[ds][qs][j]);
+          }
+      }
     }
   };
 
@@ -314,21 +356,29 @@ void attn_tree_k(TreeArgs a) {
     const short* const vt = kt + TR * U;
     const int* const pt = &spos[POS ? st : 0][w][0];
     if (k0 + TR <= c) {
+      if constexpr (TK >= 32 && ES == 2) {
 #pragma unroll
-      for (int hr = 0; hr < TK; hr += 32) {
-        const f32x4 x = scores(std::false_type{}, k0, h0 + hr, kt, pt);
-        if constexpr (TK >= 32) {
-          const f32x4 y = scores(std::false_type{}, k0, h0 + hr + 16, kt, pt);
-          product(std::integral_constant<int, 32>{}, h0 + hr, x, y, vt);
-        } else {
-          product(std::integral_constant<int, 16>{}, h0 + hr, x, x, vt);
+        for (int hr = 0; hr < TK; hr += 32) {
+          f32x4 x[QT], y[QT];
+          scores(std::false_type{}, k0, h0 + hr, kt, pt, x);
+          scores(std::false_type{}, k0, h0 + hr + 16, kt, pt, y);
+          product32(h0 + hr, x, y, vt);
+        }
+      } else {
+#pragma unroll
+        for (int hr = 0; hr < TK; hr += 16) {
+          f32x4 x[QT];
+          scores(std::false_type{}, k0, h0 + hr, kt, pt, x);
+          product16(h0 + hr, x, vt);
         }
       }
     } else {
       for (int hr = h0; hr < h0 + TK; hr += 16) {
-        const f32x4 x = scores(std::true_type{}, k0, hr, kt, pt);
+        f32x4 x[QT];
+        scores(std::true_type{}, k0, hr, kt, pt, x);
         // values that some query must not see may be anything, and 0 x inf is
-        // not 0: rows that hold a value that is not finite go one by one
+        // not 0: rows that hold a value that is not finite go one by one. (An
+        // infinity in a row of the context, which every token sees, gives NaN.)
         bool odd = false;
 #pragma unroll
         for (int u = 0; u < U / 32; ++u) {
@@ -336,54 +386,65 @@ void attn_tree_k(TreeArgs a) {
 #pragma unroll
           for (int e = 0; e < 16 / ES; ++e) odd = odd || !(fabsf((float)z.v[e]) <= 3.4028234e38f);
         }
-        if (__builtin_amdgcn_ballot_w64(odd) == 0ull) product(std::integral_constant<int, 16>{}, hr, x, x, vt);
+        if (__builtin_amdgcn_ballot_w64(odd) == 0ull) product16(hr, x, vt);
         else product_checked(hr, x, vt);
       }
     }
   }
 
   // L: over the lane groups; then, with the sums, over the row groups in order
-  lsum += __shfl_xor(lsum, 16, 64);
-  lsum += __shfl_xor(lsum, 32, 64);
-  const bool absent = anc == 0ull;
   const bool whole = a.splits == 1;
-  const int64_t prow = ((int64_t)bh * a.splits + split) * N + qi;
-  T* const op = (T*)a.o + b * a.so[0] + h * a.so[1] + qi * a.so[2];
-  float l = lsum;
   f32x4* const sx = reinterpret_cast<f32x4*>(ring);
+#pragma unroll
+  for (int qs = 0; qs < QT; ++qs) {
+    lsum[qs] += __shfl_xor(lsum[qs], 16, 64);
+    lsum[qs] += __shfl_xor(lsum[qs], 32, 64);
+    if (KG > 1 && g == 0) sl[w][16 * qs + li] = lsum[qs];
+  }
   if constexpr (KG > 1) {
-    if (g == 0) sl[w][li] = lsum;
     __syncthreads();  // the ring is idle
 #pragma unroll
-    for (int ds = 0; ds < DS; ++ds) sx[(w * DS + ds) * 64 + lane] = oacc[ds];
+    for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+      for (int qs = 0; qs < QT; ++qs) sx[((w * DS + ds) * QT + qs) * 64 + lane] = oacc[ds][qs];
     __syncthreads();
-    l = 0.f;
-#pragma unroll
-    for (int i = 0; i < KG; ++i) l += sl[i * QG + qg][li];
-  }
-  if (absent) l = 0.f;
-  const float inv = 1.f / (l + 16.f * a.eps);
-  if (qi >= N) return;
-  if (kg == 0 && g == 0) {
-    if (!whole) a.lpart[prow] = l;
-    else if (a.L) a.L[(int64_t)bh * N + qi] = l * 0.0625f;
   }
 #pragma unroll
-  for (int ds = 0; ds < DS; ++ds) {
-    if (KG > 1 && ds % KG != kg) continue;  // a row group writes every KG-th subtile
-    f32x4 t = oacc[ds];
+  for (int qs = 0; qs < QT; ++qs) {
+    const int i = qi + 16 * qs;
+    float l = lsum[qs];
     if constexpr (KG > 1) {
-      t = sx[(qg * DS + ds) * 64 + lane];
+      l = 0.f;
 #pragma unroll
-      for (int i = 1; i < KG; ++i) t += sx[((i * QG + qg) * DS + ds) * 64 + lane];
+      for (int r = 0; r < KG; ++r) l += sl[r * QG + qg][16 * qs + li];
     }
-    if (absent) t = f32x4{0.f, 0.f, 0.f, 0.f};  // (its products with rows it does not see may be NaN)
-    const int d = 16 * ds + 4 * g;
-    if (!whole) {
-      *reinterpret_cast<f32x4*>(a.part + prow * W + d) = t;
-    } else if (d < a.D) {
-      const float y[4] = {t[0] * inv, t[1] * inv, t[2] * inv, t[3] * inv};
-      store_acc<T, 4>(op + d, y);
+    const bool absent = anc[qs] == 0ull;
+    if (absent) l = 0.f;
+    const float inv = 1.f / (l + 16.f * a.eps);
+    if (i >= N) continue;
+    const int64_t prow = ((int64_t)bh * a.splits + split) * N + i;
+    T* const op = (T*)a.o + b * a.so[0] + h * a.so[1] + i * a.so[2];
+    if (kg == 0 && g == 0) {
+      if (!whole) a.lpart[prow] = l;
+      else if (a.L) a.L[(int64_t)bh * N + i] = l * 0.0625f;
+    }
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) {
+      if (KG > 1 && ds % KG != kg) continue;  // a row group writes every KG-th subtile
+      f32x4 t = oacc[ds][qs];
+      if constexpr (KG > 1) {
+        t = sx[((qg * DS + ds) * QT + qs) * 64 + lane];
+#pragma unroll
+        for (int r = 1; r < KG; ++r) t += sx[(((r * QG + qg) * DS + ds) * QT + qs) * 64 + lane];
+      }
+      if (absent) t = f32x4{0.f, 0.f, 0.f, 0.f};  // (its products with rows it does not see may be NaN)
+      const int d = 16 * ds + 4 * g;
+      if (!whole) {
+        *reinterpret_cast<f32x4*>(a.part + prow * W + d) = t;
+      } else if (d < a.D) {
+        const float y[4] = {t[0] * inv, t[1] * inv, t[2] * inv, t[3] * inv};
+        store_acc<T, 4>(op + d, y);
+      }
     }
   }
 }
@@ -441,14 +502,14 @@ template <typename T, int W> __global__ __launch_bounds__(kTreeCombThreads) void
 // T=1999, D=96: 8 splits 16.8 us, 12, past what fits, 23.5; 4 splits 20.0), none
 // without a tile.
 static int tree_splits(int64_t B, int64_t H, int64_t N, int64_t T, int W, int dtype) {
-  const TreeShape s = tree_shape(W * dtype_size(dtype) / 2, tree_qg(N));
+  const TreeShape s = tree_shape(W * dtype_size(dtype) / 2, tree_nq(N));
   const int64_t want = s.blocks * (int64_t)num_cus() / (B * H);
   return (int)std::max<int64_t>(1, std::min<int64_t>(want, (T + s.rows - 1) / s.rows));
 }
 
-template <typename T, int W, int QG, bool POS> static int launch_tree(const TreeArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((attn_tree_k<T, W, QG, POS>), dim3((unsigned)a.splits, (unsigned)(a.B * a.H)),
-                     dim3(64 * tree_at<T, W, QG>().waves), 0, st, a);
+template <typename T, int W, int NQ, bool POS> static int launch_tree(const TreeArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((attn_tree_k<T, W, NQ, POS>), dim3((unsigned)a.splits, (unsigned)(a.B * a.H)),
+                     dim3(64 * tree_at<T, W, NQ>().waves), 0, st, a);
   if (int rc = check_launch("kat_attn_tree")) return rc;
   if (a.splits == 1) return KAT_OK;
   const int64_t rows = (int64_t)a.B * a.H * a.N, rpb = kTreeCombThreads / (W / 4);
@@ -458,7 +519,7 @@ template <typename T, int W, int QG, bool POS> static int launch_tree(const Tree
 }
 template <typename T, int W> static int tree_n(const TreeArgs& a, hipStream_t st) {
   const bool pos = a.positions != nullptr;
-  switch (tree_qg(a.N)) {
+  switch (tree_nq(a.N)) {
     case 1: return pos ? launch_tree<T, W, 1, true>(a, st) : launch_tree<T, W, 1, false>(a, st);
     case 2: return pos ? launch_tree<T, W, 2, true>(a, st) : launch_tree<T, W, 2, false>(a, st);
     default: return pos ? launch_tree<T, W, 4, true>(a, st) : launch_tree<T, W, 4, false>(a, st);
