@@ -381,8 +381,8 @@ void attn_tree_k(TreeArgs a) {
         // infinity in a row of the context, which every token sees, gives NaN.)
         bool odd = false;
 #pragma unroll
-        for (int u = 0; u < U / 32; ++u) {
-          const VecT<T, 16 / ES> z = __builtin_bit_cast(VecT<T, 16 / ES>, lds16(vt + (hr + li) * U + 8 * (4 * u + g)));
+        for (int u = 0; u < U / 32; ++u) {  // (the rows as they lie, 1 KB at a time: no bank conflicts)
+          const VecT<T, 16 / ES> z = __builtin_bit_cast(VecT<T, 16 / ES>, lds16(vt + hr * U + 8 * (64 * u + lane)));
 #pragma unroll
           for (int e = 0; e < 16 / ES; ++e) odd = odd || !(fabsf((float)z.v[e]) <= 3.4028234e38f);
         }
