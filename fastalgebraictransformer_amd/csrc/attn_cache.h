@@ -47,15 +47,6 @@ template <typename T> __device__ __forceinline__ mfma::f32x4 dot64(const mfma::i
   }
 }
 
-// c += A B over 16 k-indices (v_mfma_f32_16x16x16): lane (g, li) holds A[li][4 g
-// + j] and B[4 g + j][li]
-template <typename T> __device__ __forceinline__ mfma::f32x4 mma_k16(const mfma::i16x4& a, const mfma::i16x4& b,
-                                                                    const mfma::f32x4& c) {
-  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-  if constexpr (__is_same(T, bf16)) return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
-  else return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
-}
-
 // Layout width of a head dim in the kernels over a cache: the width of its
 // columns padded to 32 (fp32 only), 64, 128 or 256; 0 if none serves (16-bit
 // types: multiples of 8 up to 256; fp32: multiples of 4 up to 128 -- the sets

@@ -50,10 +50,11 @@ template <typename T, int W> constexpr int kw_units() { return W * (int)sizeof(T
 template <int U> constexpr int kw_rows() { return U == 512 ? 32 : 64; }
 
 // KS: 16-key subtiles per wave (their fragments take U / 8 registers each). QW > 1:
-// the block's QW waves share their keys and split a tile's queries (16 rows each)
-template <typename T, int W, bool KM, int KS, int QW>
+// the block's QW waves share their keys and split a tile's queries (16 rows each).
+// KK: 64-byte column blocks that hold columns (the tiles are U / 32 wide)
+template <typename T, int W, int KK, bool KM, int KS, int QW>
 __global__ __launch_bounds__(64 * (QW > 1 ? QW : kKwWaves), (kw_units<T, W>() == 512 ? 1 : 2)) void attn_keyw_k(KeywArgs a) {
-  constexpr int ES = (int)sizeof(T), U = kw_units<T, W>(), KK = U / 32, NW = QW > 1 ? QW : kKwWaves, QR = QW > 1 ? 16 * QW : kw_rows<U>();
+  constexpr int ES = (int)sizeof(T), U = kw_units<T, W>(), NW = QW > 1 ? QW : kKwWaves, QR = QW > 1 ? 16 * QW : kw_rows<U>();
   constexpr int KWV = NW / QW;   // waves with keys of their own
   constexpr int BK = 16 * KS * KWV;    // keys per block
   constexpr int WR = QR / QW;          // rows of a tile per wave
@@ -83,6 +84,33 @@ __global__ __launch_bounds__(64 * (QW > 1 ? QW : kKwWaves), (kw_units<T, W>() ==
   // (a scale below 2^-60 moves no score, but the bias is divided by it)
   const float scale = !kBiasC || fabsf(a.scale) >= 0x1p-60f ? a.scale : copysignf(0x1p-60f, a.scale);
   const int cols = a.D * ES / 16;
+  // A block whose keys all are dropped is done (every wave reads all of its keys'
+  // mask, so they agree), and a wave without a key that counts (!live) only loads.
+  // With tiles skipped whose queries all are dropped, prompts padded on the left by
+  // 0 .. T/2 tokens: fp16, 120 heads, T=2217 107 us without, 77 with; fp32, 12 heads,
+  // T=1000 18.9 / 10.5; bf16, 48 heads, T=256, 64 queries 3.7 / 4.0. (The test after
+  // the first loads are issued: 82.5 / 11.9 / 3.9.)
+  bool live = true;
+  if constexpr (KM) {
+    uint64_t in = 0;
+    live = false;
+#pragma unroll
+    for (int i = 0; i < BK; i += 64) {
+      const int key = kb * BK + i + lane;
+      const uint64_t m = __builtin_amdgcn_ballot_w64(i + lane < BK && key < T_ && mp[std::min(key, T_ - 1)] != 0);
+      in |= m;
+      const int k0 = kw - kb * BK - i;  // the wave's keys are bits k0 .. k0 + 16 KS - 1 of one of these words
+      if (k0 >= 0 && k0 < 64) live = (m >> k0 & (1ull << 16 * KS) - 1) != 0;
+    }
+    if (in == 0) {
+      const int key = kb * BK + (int)threadIdx.x;
+      if ((int)threadIdx.x < BK && key < T_) {
+        if (a.part) a.part[((int64_t)blockIdx.y * a.B * a.H + bh) * T_ + key] = 0.f;
+        else a.out[b * a.so[0] + h * a.so[1] + key] = 0.f;
+      }
+      return;
+    }
+  }
 
   TileDma<U, NW, QR> dq;
   dq.init(w, lane, (uint32_t)(sqb / 2), a.D * ES / 2);
@@ -168,9 +196,14 @@ __global__ __launch_bounds__(64 * (QW > 1 ? QW : kKwWaves), (kw_units<T, W>() ==
     }
     const int rw = row + w0;
     if (rw + WR - 1 >= kw) {  // else every key of the wave lies past its queries
-      bool plain = rw >= kw + 16 * KS - 1;
-      if constexpr (KM) plain = plain && __builtin_amdgcn_ballot_w64(lane < WR && sc[buf][w0 + lane % WR] == 0.f) == 0ull;
-      if (plain) tile(std::false_type{}, rw, sq[buf] + w0 * U, sc[buf] + w0);
+      bool plain = rw >= kw + 16 * KS - 1, some = true;
+      if constexpr (KM) {
+        const uint64_t out = __builtin_amdgcn_ballot_w64(sc[buf][w0 + lane % WR] == 0.f);
+        plain = plain && out == 0;
+        some = live && out != ~0ull;
+      }
+      if (!some) {  // a dropped key, or queries that do not count: no weight
+      } else if (plain) tile(std::false_type{}, rw, sq[buf] + w0 * U, sc[buf] + w0);
       else tile(std::true_type{}, rw, sq[buf] + w0 * U, sc[buf] + w0);
     }
     if (more && threadIdx.x < QR) sc[buf ^ 1][threadIdx.x] = cn;
@@ -275,32 +308,44 @@ static KeywPlan keyw_plan(int64_t B, int64_t H, int64_t T, int64_t lo, int W, in
   return p;
 }
 
-template <typename T, int W, int KS, int QW> static int launch_keyw(const KeywArgs& a, hipStream_t st) {
+template <typename T, int W, int KK, int KS, int QW> static int launch_keyw(const KeywArgs& a, hipStream_t st) {
   constexpr int BK = 16 * KS * (QW > 1 ? 1 : kKwWaves);
-  const dim3 grid((unsigned)((a.T + BK - 1) / BK * a.B * a.H), (unsigned)a.chunks);
-  if (a.mask) hipLaunchKernelGGL((attn_keyw_k<T, W, true, KS, QW>), grid, dim3(64 * (QW > 1 ? QW : kKwWaves)), 0, st, a);
-  else hipLaunchKernelGGL((attn_keyw_k<T, W, false, KS, QW>), grid, dim3(64 * (QW > 1 ? QW : kKwWaves)), 0, st, a);
+  const dim3 grid((unsigned)((a.T + BK - 1) / BK * a.B * a.H), (unsigned)a.chunks), block(64 * (QW > 1 ? QW : kKwWaves));
+  if (a.mask) hipLaunchKernelGGL((attn_keyw_k<T, W, KK, true, KS, QW>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((attn_keyw_k<T, W, KK, false, KS, QW>), grid, block, 0, st, a);
   if (int rc = check_launch("kat_attn_key_weights")) return rc;
   if (!a.part) return KAT_OK;
   hipLaunchKernelGGL(attn_keyw_sum_k, dim3((unsigned)((a.T + 255) / 256), (unsigned)(a.B * a.H)), dim3(256), 0, st, a, BK);
   return check_launch("kat_attn_key_weights (sum)");
 }
-template <typename T, int W> static int keyw_mode(const KeywArgs& a, const KeywPlan& p, hipStream_t st) {
+template <typename T, int W, int KK> static int keyw_mode(const KeywArgs& a, const KeywPlan& p, hipStream_t st) {
   if constexpr (kw_units<T, W>() <= 256) {
-    if (p.qw == 8) return launch_keyw<T, W, 1, 8>(a, st);
+    if (p.qw == 8) return launch_keyw<T, W, KK, 1, 8>(a, st);
   }
-  if (p.qw == 4) return launch_keyw<T, W, 1, 4>(a, st);
+  if (p.qw == 4) return launch_keyw<T, W, KK, 1, 4>(a, st);
   if constexpr (sizeof(T) == 2) {
-    if (p.ks == 2) return launch_keyw<T, W, 2, 1>(a, st);
+    if (p.ks == 2) return launch_keyw<T, W, KK, 2, 1>(a, st);
   }
-  return launch_keyw<T, W, 1, 1>(a, st);
+  return launch_keyw<T, W, KK, 1, 1>(a, st);
+}
+// Column blocks: all of a layout's, or the first three quarters where the head
+// dim ends there (96, 192; 48 in fp32), so that no zeros are multiplied. All / three
+// quarters, us: fp32, 128 heads, T=1245, D=80 246 / 203; fp32, 144 heads, T=2048,
+// D=48 355 / 295; bf16, 64 heads, T=2048, D=96 64.6 / 58.1; bf16, 48 heads, T=1000,
+// D=192 24.1 / 22.2.
+template <typename T, int W> static int keyw_cols(const KeywArgs& a, const KeywPlan& p, hipStream_t st) {
+  constexpr int KK = kw_units<T, W>() / 32;
+  if constexpr (KK >= 4) {
+    if (a.D <= W / 4 * 3) return keyw_mode<T, W, KK / 4 * 3>(a, p, st);
+  }
+  return keyw_mode<T, W, KK>(a, p, st);
 }
 template <typename T> static int keyw_w(const KeywArgs& a, int W, const KeywPlan& p, hipStream_t st) {
   switch (W) {
-    case 32: if constexpr (sizeof(T) == 4) return keyw_mode<T, 32>(a, p, st); break;
-    case 64: return keyw_mode<T, 64>(a, p, st);
-    case 128: return keyw_mode<T, 128>(a, p, st);
-    case 256: return keyw_mode<T, 256>(a, p, st);
+    case 32: if constexpr (sizeof(T) == 4) return keyw_cols<T, 32>(a, p, st); break;
+    case 64: return keyw_cols<T, 64>(a, p, st);
+    case 128: return keyw_cols<T, 128>(a, p, st);
+    case 256: return keyw_cols<T, 256>(a, p, st);
   }
   return fail(KAT_EUNSUPPORTED, "kat_attn_key_weights: head dim %d", a.D);
 }

@@ -367,6 +367,43 @@ def test_key_weights_with_dropped_tokens(gpu, dtype, D):
                 assert float(w[b, h][~mask[b].to(dev)].abs().sum()) == 0
 
 
+# one call per way a grid is laid out, at head dims that end in the third quarter of
+# their layout's columns and at full ones
+@pytest.mark.parametrize("dtype,B,H,T,D", [
+    (torch.bfloat16, 6, 2, 200, 96), (torch.float16, 12, 4, 333, 40), (torch.float32, 6, 12, 256, 48),
+    (torch.bfloat16, 6, 1, 1301, 80), (torch.float32, 6, 1, 1301, 96), (torch.float32, 18, 16, 130, 80),
+    (torch.float16, 60, 12, 257, 128), (torch.bfloat16, 60, 12, 257, 192), (torch.float32, 6, 2, 300, 160),
+    (torch.float32, 6, 2, 300, 256)])
+def test_key_weights_with_runs_of_dropped_tokens(gpu, dtype, B, H, T, D):
+    q, k = rand((B, H, T, D), dtype, 11), rand((B, H, T, D), dtype, 12)
+    mask = torch.ones(B, T, dtype=torch.bool)
+    for b in range(B):
+        if b % 6 == 0: mask[b, :2 * T // 3] = False              # left padding
+        elif b % 6 == 1: mask[b, T // 4:] = False                # right padding
+        elif b % 6 == 2: mask[b, 5:T - 7] = False                # only the ends
+        elif b % 6 == 3: mask[b, T // 5:T // 5 + 1 + 3 * T // 8] = False  # a hole
+        elif b % 6 == 4: mask[b] = False
+    slopes = F.compute_alibi_slopes(H)
+    L = torch.rand(B, H, T, generator=torch.Generator().manual_seed(13)) + 0.5
+    q2, k2, L2 = q.clone(), k.clone(), L.clone()
+    for b in range(B):
+        q2[b, :, ~mask[b].to(dev)] = float("inf")
+        k2[b, :, ~mask[b].to(dev)] = float("nan")
+        L2[b, :, ~mask[b]] = float("nan")
+    for last in (None, T // 3):
+        w = F.rational_attention_key_weights(q2, k2, slopes.to(dev), 0.1, L2.to(dev), key_mask=mask.to(dev), last=last)
+        torch.cuda.synchronize()
+        for b in range(6):
+            for h in {0, H - 1}:
+                ref, tol = C.key_weights(q[b, h].cpu(), k[b, h].cpu(), slopes[h], 0.1, L[b, h], mask[b], last)
+                err = (w[b, h].double().cpu() - ref).abs()
+                assert bool((err <= tol + 1e-30).all()), (b, h, last, float((err - tol).max()))
+        assert float(w.masked_select(~mask.to(dev)[:, None].expand(B, H, T)).abs().sum()) == 0
+        for b in range(6, B):  # the other rows: finite, and not zero where a query counts
+            assert bool(torch.isfinite(w[b]).all())
+            assert bool((w[b].sum(-1) > 0).all()) == bool(mask[b, T - (last or T):].any())
+
+
 @pytest.mark.parametrize("B,H,T", [(1, 2, 2500), (8, 16, 700)])
 def test_key_weights_of_split_and_full_grids(gpu, B, H, T):
     # grids that split the queries and grids that do not: rows add up to the
