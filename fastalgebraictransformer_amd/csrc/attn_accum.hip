@@ -211,16 +211,15 @@ template <typename T, int W> __global__ __launch_bounds__(kAccThreads) void attn
   float t[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const int col = threadIdx.x;
   const bool first = blockIdx.x == 0;
-  if (first && col < W) {
+  if (first && col < W) {  // (a missing split loads the last one again: no branch between the loads)
     const float* p = a.part + (int64_t)bh * S * W + col;
-    int s = 0;
-    for (; s + 8 <= S; s += 8) {
+    for (int s = 0; s < S; s += 8) {
+      float x[8];
 #pragma unroll
-      for (int r = 0; r < 8; ++r) t[r] += p[(int64_t)(s + r) * W];
+      for (int r = 0; r < 8; ++r) x[r] = p[(int64_t)min(s + r, S - 1) * W];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) t[r] += s + r < S ? x[r] : 0.f;
     }
-#pragma unroll
-    for (int r = 0; r < 7; ++r)
-      if (s + r < S) t[r] += p[(int64_t)(s + r) * W];
   }
   int n = a.lengths ? a.lengths[b] : a.T;
   n = min(max(n, 0), a.T);

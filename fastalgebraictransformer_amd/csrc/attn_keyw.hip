@@ -234,7 +234,8 @@ __global__ __launch_bounds__(64 * (QW > 1 ? QW : kKwWaves), (kw_units<T, W>() ==
   }
 }
 
-// adds the chunks of each key in order
+// adds the chunks of each key in order (a missing chunk loads the last one again:
+// no branch between the loads)
 __global__ __launch_bounds__(256) void attn_keyw_sum_k(KeywArgs a, int bk) {
   const int bh = blockIdx.y, b = bh / a.H, h = bh - b * a.H;
   const int key = blockIdx.x * 256 + threadIdx.x;
@@ -244,14 +245,13 @@ __global__ __launch_bounds__(256) void attn_keyw_sum_k(KeywArgs a, int bk) {
   const int64_t step = (int64_t)a.B * a.H * a.T;
   const float* p = a.part + (int64_t)bh * a.T + key;
   float t[4] = {0.f, 0.f, 0.f, 0.f};
-  int c = 0;
-  for (; c + 4 <= nc; c += 4) {
+  for (int c = 0; c < nc; c += 4) {
+    float x[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) t[r] += p[(c + r) * step];
+    for (int r = 0; r < 4; ++r) x[r] = p[std::min(c + r, nc - 1) * step];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) t[r] += c + r < nc ? x[r] : 0.f;
   }
-#pragma unroll
-  for (int r = 0; r < 3; ++r)
-    if (c + r < nc) t[r] += p[(c + r) * step];
   a.out[b * a.so[0] + h * a.so[1] + key] = (t[0] + t[1]) + (t[2] + t[3]);
 }
 

@@ -451,7 +451,9 @@ void attn_tree_k(TreeArgs a) {
 
 // o = sum over the splits / (L + eps): a thread per 4 columns of a query row,
 // eight independent loads in flight, added in split order in eight running sums
-// (deterministic)
+// (deterministic). The last splits load as the others do, a missing one the last
+// split again: with a branch around each they waited in turn, up to a microsecond
+// a load (bf16, 12 heads, 57 tokens, T=2016: D=64 15.9 -> 14.0 us, D=128 20.6 -> 18.8)
 constexpr int kTreeCombThreads = 256;
 template <typename T, int W> __global__ __launch_bounds__(kTreeCombThreads) void attn_tree_combine_k(TreeArgs a) {
   constexpr int TPR = W / 4, RPB = kTreeCombThreads / TPR;  // threads per row, rows per block
@@ -468,22 +470,23 @@ template <typename T, int W> __global__ __launch_bounds__(kTreeCombThreads) void
     t[r] = f32x4{0.f, 0.f, 0.f, 0.f};
     l[r] = 0.f;
   }
-  int s = 0;
-  for (; s + 8 <= a.splits; s += 8) {
+  for (int s = 0; s < a.splits; s += 8) {
+    f32x4 x[8];
+    float y[8];
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-      const int64_t p = p0 + (int64_t)(s + r) * a.N;
-      t[r] += *reinterpret_cast<const f32x4*>(a.part + p * W + d);
-      l[r] += a.lpart[p];
+      const int64_t p = p0 + (int64_t)std::min(s + r, a.splits - 1) * a.N;
+      x[r] = *reinterpret_cast<const f32x4*>(a.part + p * W + d);
+      y[r] = a.lpart[p];
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const bool in = s + r < a.splits;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t[r][j] += in ? x[r][j] : 0.f;
+      l[r] += in ? y[r] : 0.f;
     }
   }
-#pragma unroll
-  for (int r = 0; r < 7; ++r)
-    if (s + r < a.splits) {
-      const int64_t p = p0 + (int64_t)(s + r) * a.N;
-      t[r] += *reinterpret_cast<const f32x4*>(a.part + p * W + d);
-      l[r] += a.lpart[p];
-    }
   const f32x4 x = ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
   const float y = ((l[0] + l[1]) + (l[2] + l[3])) + ((l[4] + l[5]) + (l[6] + l[7]));
   if (d == 0 && a.L) a.L[row] = y * 0.0625f;
