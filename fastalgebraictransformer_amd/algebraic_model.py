@@ -416,16 +416,22 @@ class AlgebraicTransformerLM(nn.Module):
         parents = parents.to(device=tokens.device, dtype=torch.int32).expand(B, N)
         positions = None
         if caches[0].keep is not None:
-            i = torch.arange(N, device=tokens.device)
-            up = (parents[:, :, None] == i).float() + torch.eye(N, device=tokens.device)
-            depth = (torch.linalg.matrix_power(up, 64) > 0).sum(-1) - 1  # ancestors above each token
-            positions = (depth + (n if position is None else position)).to(torch.int32)
+            positions = (self._depths(parents) + (n if position is None else position)).to(torch.int32)
         x = self.embed(tokens)
         r = None
         for block, cache in zip(self.blocks, caches):
             x, r = block.tree_pending(x, r, cache, parents, n, lengths, positions)
         _, normed = add_mean_error_norm(x, r, self.norm.weight, self.norm.eps, _narrow(x))
         return self.head(normed)
+
+    @staticmethod
+    def _depths(parents: torch.Tensor) -> torch.Tensor:
+        """How many drafted tokens stand above each one of parents [B, N]."""
+        N = parents.size(1)
+        with torch.autocast(parents.device.type, enabled=False):  # counts of paths pass fp16's range
+            i = torch.arange(N, device=parents.device)
+            up = (parents[:, :, None] == i).float() + torch.eye(N, device=parents.device)
+            return (torch.linalg.matrix_power(up, 64) > 0).sum(-1) - 1
 
     @staticmethod
     def accept_drafted(caches, n: int, path: torch.Tensor):

@@ -147,3 +147,19 @@ def test_workspaces_are_bounded(B, H, T):
     assert lib.kat_attn_tree_workspace_size(B, H, 64, T, 128, 1) <= max(cache, 64 << 20)
     assert lib.kat_attn_decode_accum_workspace_size(B, H, T, 128, 1) <= max(cache // 8, 8 << 20)
     assert lib.kat_attn_key_weights_workspace_size(B, H, T, 128, 64, 1) <= max(cache // 8, 8 << 20)
+
+
+@pytest.mark.parametrize("dtype", [None, torch.bfloat16, torch.float16])
+def test_depths_of_drafted_tokens_under_autocast(dtype):
+    from fastalgebraictransformer_amd.algebraic_model import AlgebraicTransformerLM
+    g = torch.Generator().manual_seed(0)
+    chain = torch.arange(64) - 1
+    tree = torch.tensor([-1] + [int(torch.randint(-1, i, (1,), generator=g)) for i in range(1, 64)])
+    parents = torch.stack((chain, tree, torch.full((64,), -1))).to(torch.int32)
+    want = torch.zeros_like(parents)
+    for b in range(3):
+        for i in range(64):
+            want[b, i] = 0 if parents[b, i] < 0 else want[b, int(parents[b, i])] + 1
+    with torch.autocast("cpu", dtype=dtype or torch.bfloat16, enabled=dtype is not None):
+        got = AlgebraicTransformerLM._depths(parents)
+    assert torch.equal(got, want.long())
