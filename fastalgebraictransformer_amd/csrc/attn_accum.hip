@@ -170,7 +170,7 @@ __global__ __launch_bounds__(64 * (ONE ? kOneWaves : kAccWaves)) void attn_accum
     l = 0.f;
 #pragma unroll
     for (int ww = 0; ww < NW; ++ww) l += sh_l[ww];
-    const float inv = 1.f / (l + 16.f * a.eps);
+    const float inv = inv_sum(l + 16.f * a.eps);
     if (threadIdx.x == 0 && a.L) a.L[bh] = l * 0.0625f;
     if ((int)threadIdx.x < a.D) {
       float t = 0.f;
@@ -237,7 +237,7 @@ template <typename T, int W> __global__ __launch_bounds__(kAccThreads) void attn
   }
   __syncthreads();
   l = (sh[0] + sh[1]) + (sh[2] + sh[3]);
-  const float inv = 1.f / (l + 16.f * a.eps);
+  const float inv = inv_sum(l + 16.f * a.eps);
   if (first) {
     if (col == 0 && a.L) a.L[bh] = l * 0.0625f;
     if (col < a.D)

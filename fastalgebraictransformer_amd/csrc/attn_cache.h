@@ -47,6 +47,9 @@ template <typename T> __device__ __forceinline__ mfma::f32x4 dot64(const mfma::i
   }
 }
 
+// 1 / d; 0 for a row sum of 0 with eps = 0, whose numerators are 0 too
+__device__ __forceinline__ float inv_sum(float d) { return d != 0.f ? 1.f / d : 0.f; }
+
 // Layout width of a head dim in the kernels over a cache: the width of its
 // columns padded to 32 (fp32 only), 64, 128 or 256; 0 if none serves (16-bit
 // types: multiples of 8 up to 256; fp32: multiples of 4 up to 128 -- the sets

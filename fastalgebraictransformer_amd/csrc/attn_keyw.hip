@@ -121,7 +121,7 @@ __global__ __launch_bounds__(64 * (QW > 1 ? QW : kKwWaves), (kw_units<T, W>() ==
   auto cinv = [&](int row) __attribute__((always_inline)) {
     const bool in = row < r1 && (!KM || mp[std::min(row, T_ - 1)] != 0);
     const float l = lp[(int64_t)std::min(row, T_ - 1) * a.sl[2]];
-    return in ? 1.f / (16.f * (l + a.eps)) : 0.f;
+    return in ? inv_sum(16.f * (l + a.eps)) : 0.f;
   };
 
   issue(sq[0], r0);

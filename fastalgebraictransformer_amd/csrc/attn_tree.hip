@@ -420,7 +420,7 @@ void attn_tree_k(TreeArgs a) {
     }
     const bool absent = anc[qs] == 0ull;
     if (absent) l = 0.f;
-    const float inv = 1.f / (l + 16.f * a.eps);
+    const float inv = inv_sum(l + 16.f * a.eps);
     if (i >= N) continue;
     const int64_t prow = ((int64_t)bh * a.splits + split) * N + i;
     T* const op = (T*)a.o + b * a.so[0] + h * a.so[1] + i * a.so[2];
@@ -491,7 +491,7 @@ template <typename T, int W> __global__ __launch_bounds__(kTreeCombThreads) void
   const float y = ((l[0] + l[1]) + (l[2] + l[3])) + ((l[4] + l[5]) + (l[6] + l[7]));
   if (d == 0 && a.L) a.L[row] = y * 0.0625f;
   if (d < a.D) {
-    const float inv = 1.f / (y + 16.f * a.eps);
+    const float inv = inv_sum(y + 16.f * a.eps);
     const float z[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
     store_acc<T, 4>((T*)a.o + b * a.so[0] + h * a.so[1] + i * a.so[2] + d, z);
   }

@@ -229,6 +229,24 @@ def test_refused_arguments(gpu):
     assert torch.equal(c.total, c.first) and c.n.tolist() == [T, T - 7]  # nothing was written
 
 
+@pytest.mark.parametrize("T", [70, 5000])
+def test_rows_without_keys_are_zero_with_eps_0(gpu, T):
+    B, H, D, N = 2, 2, 64, 5
+    q, k, v = (rand((B, H, n, D), torch.bfloat16, s) for n, s in ((N, 1), (T, 2), (T, 3)))
+    slopes = torch.tensor([0.5, 0.1], device=dev)
+    parents = torch.tensor([-1, 0, -7, 2, 1], dtype=torch.int32, device=dev)  # 2 and, below it, 3 are absent
+    n = torch.tensor([T, N - 1], dtype=torch.int32, device=dev)               # row 1: no room for the tokens
+    o, L = F.rational_attention_tree(q, k, v, slopes, 0.125, parents, lengths=n, eps=0.0)
+    assert float(o[0, :, 2:4].abs().max()) == 0 and float(o[1].abs().max()) == 0 and float(L[1].abs().max()) == 0
+    assert bool(torch.isfinite(o).all()) and float(o[0, :, 4].abs().max()) > 0
+    n[1] = 0
+    total = rand((B, H, T), torch.float32, 4)
+    before = total.clone()
+    o, L = F.rational_attention_decode_accumulate(q[:, :, 0], k, v, slopes, 0.125, total, lengths=n, eps=0.0)
+    assert float(o[1].abs().max()) == 0 and float(L[1].abs().max()) == 0 and torch.equal(total[1], before[1])
+    assert bool(torch.isfinite(o).all()) and bool((total[0] >= before[0]).all())
+
+
 def test_caches_past_2_31_bytes(gpu):
     # one head of a wide token-major cache: rows 64 KB apart, the last past 2^31
     T, heads, D, N = 33000, 512, 64, 6
