@@ -501,13 +501,23 @@ template <typename T, int W> __global__ __launch_bounds__(kTreeCombThreads) void
 // Host side
 // ---------------------------------------------------------------------------
 
-// Blocks per (b, h): as many as the CUs hold at once and no more (B=3, H=16, N=25,
-// T=1999, D=96: 8 splits 16.8 us, 12, past what fits, 23.5; 4 splits 20.0), none
-// without a tile.
+// Blocks per (b, h): no more than the CUs hold at once (B=3, H=16, N=25, T=1999, D=96:
+// 8 splits 16.8 us, 12, past what fits, 23.5; 4 splits 20.0), none without a tile; of
+// those the number with the least time in tiles one after another and in the combine,
+// whose rounds of eight splits take about three tiles' time each. Most that fit / this
+// rule, bf16, 12 heads: N=64, D=64, T=1344 12.6 (21) / 10.9 us (8), T=4032 14.2 / 12.6
+// (16); N=57, D=256, T=4000 30.5 (21) / 25.6 (16), T=16000 52 (21, as here) against 54.6
+// (16); N=8, D=64, T=8192 13.7 (42) / 11.3 (16); one head, N=16, D=64, T=65536 47.5 (512) /
+// 17.7; four heads, N=57, D=128, T=32768 28.7 (64) / 29.6 (40).
 static int tree_splits(int64_t B, int64_t H, int64_t N, int64_t T, int W, int dtype) {
   const TreeShape s = tree_shape(W * dtype_size(dtype) / 2, tree_nq(N));
-  const int64_t want = s.blocks * (int64_t)num_cus() / (B * H);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(want, (T + s.rows - 1) / s.rows));
+  const int64_t tiles = (T + s.rows - 1) / s.rows;
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(s.blocks * (int64_t)num_cus() / (B * H), tiles));
+  auto cost = [&](int64_t n) { return (tiles + n - 1) / n + 3 * ((n + 7) / 8); };
+  int64_t best = most;
+  for (int64_t n = (most - 1) / 8 * 8; n > 0; n -= 8)
+    if (cost(n) < cost(best)) best = n;
+  return (int)best;
 }
 
 template <typename T, int W, int NQ, bool POS> static int launch_tree(const TreeArgs& a, hipStream_t st) {
